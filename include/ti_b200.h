@@ -146,6 +146,100 @@ ti_status ti_op_paged_attention_noalloc(const void* qkv, int batch, int n_heads,
                                         int pt_stride, void* k_pages, void* v_pages, int n_pages, int max_len,
                                         float theta, const ti_rope_scaling* scaling, int sliding_window, void* out,
                                         void* stream);
+/* ---- serving operators over the paged cache: rotation, append and attention
+ * for many new tokens of many sequences.  No counterpart in the reference,
+ * which rotates, copies and attends one sequence at a time (llama_model.cpp:147-182).
+ *
+ * All pointers inside the structs and arguments are device pointers; the entries
+ * select the device that holds `out` (or the pages), whatever device is current,
+ * and `stream` is a stream of that device (NULL = its legacy default stream).
+ * They allocate nothing but stream-ordered scratch, synchronise nothing and may
+ * be captured into graphs; captured graphs share no scratch.  What arrays on the
+ * device say is checked there: a token without a sequence, a position outside
+ * the page table, and a row or page id out of range read as "no such key" or
+ * are skipped, not reported. */
+
+/* Rotary positions on one to four axes (time, height, width ...).  Pair
+ * (i, i + rot_dim/2) of the first rot_dim dimensions of a head turns by
+ * pos[axis(i)][t] * inv_freq[i]; dimensions past rot_dim pass unchanged.
+ * axis(i): blocks of sections[0], sections[1], ... pairs, or, interleaved,
+ * i % n_axes while i / n_axes < sections[i % n_axes], else axis 0.
+ * The angle is exact for the fp32 frequencies and any int32 position (reduced
+ * in fp64), cosine and sine are fp32, the result is rounded once. */
+typedef struct {
+    int rot_dim;              /* even, 2 .. min(head_dim, 512) */
+    const float* inv_freq;    /* [rot_dim / 2] (ti_rope_inv_freq) */
+    int n_axes;               /* 1 .. 4 */
+    int sections[4];          /* pairs of each axis, summing to rot_dim / 2; not read when n_axes == 1 */
+    int interleaved;
+    const int32_t* pos;       /* [n_axes, pos_stride]; NULL (ti_op_kv_append, one axis): the position in the cache */
+    int64_t pos_stride;       /* entries from one axis to the next, >= the tokens */
+} ti_rope_axes;
+/* The frequency table of theta and llama3 scaling (scaling may be NULL), host
+ * memory in and out: what ti_op_rope and the engine use (ops.cu:235-278). */
+ti_status ti_rope_inv_freq(int head_dim, float theta, const ti_rope_scaling* scaling, float* out);
+/* The multi-axis form of ti_op_rope, for encoders and wherever no cache is kept:
+ * x [n_tokens, heads, head_dim] -> out, dtype BF16, F16 or F32; a token's heads are
+ * contiguous, x_stride / out_stride elements lie between tokens.  out may be x
+ * (same stride); any other overlap is not supported. */
+ti_status ti_op_rope_axes(int dtype, const void* x, int64_t x_stride, void* out, int64_t out_stride, int n_tokens,
+                          int heads, int head_dim, const ti_rope_axes* rope, void* stream);
+
+/* A layer's paged cache, as ti_op_paged_attention's: 16 tokens a page. */
+typedef struct {
+    int dtype;                  /* TI_DTYPE_BF16 or TI_DTYPE_F16: the pages, q, k, v and out */
+    int n_kv, head_dim;
+    void* k_pages;              /* [n_pages, n_kv, 16, head_dim], 16-byte aligned */
+    void* v_pages;
+    int n_pages;
+    const int32_t* page_table;  /* [table_rows, pt_stride] page ids */
+    int table_rows, pt_stride;
+} ti_paged_kv;
+/* The new tokens of a call, sequence after sequence: tokens start[s] .. start[s+1] - 1
+ * are sequence s's newest, at positions kv_len[s] - (start[s+1] - start[s]) .. kv_len[s] - 1.
+ * Tokens from start[n_seqs] on (padding) belong to nobody: nothing is written for them.
+ * Sequences without new tokens, and kv_len of zero or less (no position, no key), are fine. */
+typedef struct {
+    int n_seqs;
+    int n_tokens;               /* rows of q / k / v / out */
+    const int32_t* start;       /* [n_seqs + 1], ascending; NULL: token s is sequence s's (n_tokens == n_seqs) */
+    const int32_t* kv_len;      /* [n_seqs] positions of each sequence, the new tokens' included */
+    const int32_t* row;         /* [n_seqs] rows of the page table; NULL: row s */
+    int max_len;                /* the longest kv_len, for dividing the work (longer ones still come out right) */
+} ti_ragged;
+/* Rotate q into q_out and k into the pages at each token's position, and copy v
+ * there.  q [n_tokens, n_heads, head_dim] may be NULL (k and v only), rope may be
+ * NULL (no rotation); strides are elements between tokens (a fused q|k|v row: its
+ * width).  q_out may be q (same stride).  head_dim even, 2 .. 1024. */
+ti_status ti_op_kv_append(const ti_paged_kv* kv, const ti_ragged* batch, const ti_rope_axes* rope, const void* q,
+                          int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                          int n_heads, void* q_out, int64_t q_out_stride, void* stream);
+
+/* How scores are made from q.k and which keys a token sees.  All zero = plain causal attention.
+ *   z = scale q.k;  softcap > 0: z = softcap tanh(z / softcap);  slopes: z -= slopes[h] |i - j|
+ * for the token at position i and key j; it sees j < kv_len[s] with
+ *   j <= i or j < prefix[s],  j > i - sliding_window (when > 0),  j >= doc_start[t].
+ * A token that sees nothing gets a zero row.  K and V of positions that no token
+ * of a 256-row tile sees never enter, whatever they hold; V of a position that a
+ * neighbouring token sees must be finite. */
+typedef struct {
+    float scale;                /* 0: 1 / sqrt(head_dim) */
+    float softcap;              /* 0: none */
+    const float* slopes;        /* [n_heads]; NULL: no distance bias */
+    int sliding_window;         /* <= 0: none */
+    const int32_t* prefix;      /* [n_seqs] first positions that see each other both ways; NULL: none */
+    const int32_t* doc_start;   /* [n_tokens] lowest position a token sees (its document's first); NULL: 0 */
+} ti_attn_form;
+/* Attention of the new tokens of a ragged batch over the paged cache, which holds
+ * their own k and v already (ti_op_kv_append).  q (rotated) and out
+ * [n_tokens, n_heads, head_dim], strides in elements between tokens; form may be
+ * NULL; head_dim 64, 128 or 256; any n_heads that n_kv divides. */
+ti_status ti_op_paged_prefill(const ti_paged_kv* kv, const ti_ragged* batch, const ti_attn_form* form, const void* q,
+                              int64_t q_stride, int n_heads, void* out, int64_t out_stride, void* stream);
+/* The same for one new token a sequence (batch->start must be NULL): the cache is
+ * read once at memory speed, split over its length and joined. */
+ti_status ti_op_paged_decode(const ti_paged_kv* kv, const ti_ragged* batch, const ti_attn_form* form, const void* q,
+                             int64_t q_stride, int n_heads, void* out, int64_t out_stride, void* stream);
 /* ops.hpp:98 / ops.cu:586-616 (BF16<->F32; same dtype = copy). */
 ti_status ti_op_cast(int src_dtype, int dst_dtype, const void* x, void* out, size_t n, void* stream);
 /* ops.hpp:95 / ops.cu:559-584: 2-D transpose [rows, cols] -> [cols, rows], F32 or BF16. */

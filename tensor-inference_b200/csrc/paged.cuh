@@ -1,0 +1,124 @@
+// paged.cuh — what the ragged-batch operators over the paged cache share
+// (rotary append, prefill attention, decode attention): the kernel-side view of
+// ti_ragged / ti_paged_kv / ti_attn_form, bounds-checked look-ups, and 16-bit types.
+#pragma once
+#include "common.cuh"
+#include "internal.h"
+#include "kernels.h"
+
+namespace ti {
+
+constexpr int kPageTokens = 16;
+constexpr float kLog2E = 1.4426950408889634f;
+
+// ------------------------------------------------------------------ 16-bit element types
+template <class T>
+struct Elem;
+template <>
+struct Elem<__nv_bfloat16> {
+    static constexpr uint32_t kUmmaFmt = 1;  // tcgen05 kind::f16 operand format
+    static TI_DEVICE_INLINE float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static TI_DEVICE_INLINE __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+    static TI_DEVICE_INLINE float lo(uint32_t u) { return __uint_as_float(u << 16); }
+    static TI_DEVICE_INLINE float hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+    static TI_DEVICE_INLINE uint32_t pack(float l, float h) {
+        uint32_t d;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(h), "f"(l));
+        return d;
+    }
+};
+template <>
+struct Elem<__half> {
+    static constexpr uint32_t kUmmaFmt = 0;
+    static TI_DEVICE_INLINE float to_f(__half v) { return __half2float(v); }
+    static TI_DEVICE_INLINE __half from_f(float v) { return __float2half_rn(v); }
+    static TI_DEVICE_INLINE float lo(uint32_t u) { return __half2float(__ushort_as_half((unsigned short)(u & 0xffffu))); }
+    static TI_DEVICE_INLINE float hi(uint32_t u) { return __half2float(__ushort_as_half((unsigned short)(u >> 16))); }
+    static TI_DEVICE_INLINE uint32_t pack(float l, float h) {
+        uint32_t d;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(h), "f"(l));
+        return d;
+    }
+};
+template <>
+struct Elem<float> {
+    static TI_DEVICE_INLINE float to_f(float v) { return v; }
+    static TI_DEVICE_INLINE float from_f(float v) { return v; }
+};
+
+// ------------------------------------------------------------------ ragged batch
+struct RaggedDev {
+    int n_seqs, n_tokens;
+    const int32_t* start;   // nullptr: token s is sequence s's
+    const int32_t* kv_len;
+    const int32_t* row;     // nullptr: row s
+    const int32_t* table;
+    int table_rows, pt_stride;
+    int n_pages;
+};
+
+// first and one-past-last token of sequence s, clipped to the rows there are
+TI_DEVICE_INLINE void seq_tokens(const RaggedDev& r, int s, int& t0, int& t1) {
+    if (r.start) {
+        t0 = max(0, min(r.start[s], r.n_tokens));
+        t1 = max(t0, min(r.start[s + 1], r.n_tokens));
+    } else {
+        t0 = s;
+        t1 = s + 1;
+    }
+}
+// sequence of token t (a whole warp asks for the same t): how many sequences end
+// at or before it; n_seqs for a token that belongs to nobody
+TI_DEVICE_INLINE int seq_of_token(const RaggedDev& r, int t) {
+    if (!r.start) return t;
+    const int lane = threadIdx.x & 31;
+    int n = 0;
+    for (int i = lane; i < r.n_seqs; i += 32) n += r.start[i + 1] <= t;
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
+}
+// page-table row of sequence s, nullptr when out of range
+TI_DEVICE_INLINE const int32_t* table_row(const RaggedDev& r, int s) {
+    const int row = r.row ? r.row[s] : s;
+    return row >= 0 && row < r.table_rows ? r.table + (size_t)row * r.pt_stride : nullptr;
+}
+
+// ------------------------------------------------------------------ score form
+struct FormDev {
+    float scale;          // of q.k
+    float cap;            // 0: none
+    const float* slopes;  // [n_heads] or nullptr
+    int window;           // <= 0: none
+    const int32_t* prefix;
+    const int32_t* doc;
+};
+// keys [lo, hi) that token t at position i of sequence s sees, within n_keys keys
+TI_DEVICE_INLINE void key_range(const FormDev& f, int s, int t, int i, int n_keys, int& lo, int& hi) {
+    lo = f.window > 0 ? max(0, i - f.window + 1) : 0;
+    if (f.doc) lo = max(lo, f.doc[t]);
+    hi = i + 1;
+    if (f.prefix) hi = max(hi, f.prefix[s]);
+    hi = min(hi, n_keys);
+    if (i < 0 || hi <= lo) lo = hi = 0;
+}
+
+// ------------------------------------------------------------------ host side
+// the device that holds p (TI_ERR_INVALID for host memory)
+ti_status device_of(const void* p, const char* who, int* dev);
+ti_status check_paged(const ti_paged_kv* kv, const ti_ragged* batch, const char* who);
+RaggedDev ragged_dev(const ti_paged_kv* kv, const ti_ragged* b);
+
+struct PagedAttn {
+    RaggedDev r;
+    FormDev f;
+    const void* q;
+    int64_t q_stride;
+    void* out;
+    int64_t out_stride;
+    const void* k_pages;
+    const void* v_pages;
+    int n_heads, n_kv, hd, dtype;
+    int max_len;
+};
+
+}  // namespace ti

@@ -40,6 +40,38 @@ class RopeScaling(C.Structure):
                 ("high_freq_factor", C.c_float), ("original_max_pos", C.c_int)]
 
 
+class RopeAxes(C.Structure):
+    """ti_rope_axes: rotary positions on one to four axes (device pointers as integers)"""
+    _fields_ = [("rot_dim", C.c_int), ("inv_freq", C.c_void_p), ("n_axes", C.c_int), ("sections", C.c_int * 4),
+                ("interleaved", C.c_int), ("pos", C.c_void_p), ("pos_stride", C.c_int64)]
+
+
+class PagedKv(C.Structure):
+    """ti_paged_kv: one layer's paged cache"""
+    _fields_ = [("dtype", C.c_int), ("n_kv", C.c_int), ("head_dim", C.c_int), ("k_pages", C.c_void_p),
+                ("v_pages", C.c_void_p), ("n_pages", C.c_int), ("page_table", C.c_void_p), ("table_rows", C.c_int),
+                ("pt_stride", C.c_int)]
+
+
+class Ragged(C.Structure):
+    """ti_ragged: the new tokens of a call, sequence after sequence"""
+    _fields_ = [("n_seqs", C.c_int), ("n_tokens", C.c_int), ("start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("row", C.c_void_p), ("max_len", C.c_int)]
+
+
+class AttnForm(C.Structure):
+    """ti_attn_form: scale, tanh cap, distance bias and masks of paged attention"""
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("slopes", C.c_void_p), ("sliding_window", C.c_int),
+                ("prefix", C.c_void_p), ("doc_start", C.c_void_p)]
+
+
+def rope_inv_freq(head_dim, theta, scaling=None):
+    """the fp32 RoPE frequency table ti_op_rope and the engine use (ti_rope_inv_freq)"""
+    out = np.empty(head_dim // 2, np.float32)
+    check(lib().ti_rope_inv_freq(head_dim, theta, C.byref(scaling) if scaling else None, _ptr(out)))
+    return out
+
+
 class Sampling(C.Structure):
     """ti_sampling: the reference's Greedy / TopP / TopK options (sampling/top_p.hpp)."""
     _fields_ = [("kind", C.c_int), ("temperature", C.c_float), ("p", C.c_float), ("k", C.c_uint32),
@@ -108,6 +140,16 @@ _SIGS = {
     "ti_op_paged_attention": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
                                         C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_float,
                                         C.POINTER(RopeScaling), C.c_int, C.c_void_p, C.c_void_p]),
+    "ti_rope_inv_freq": (C.c_int, [C.c_int, C.c_float, C.POINTER(RopeScaling), C.c_void_p]),
+    "ti_op_rope_axes": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_int,
+                                  C.POINTER(RopeAxes), C.c_void_p]),
+    "ti_op_kv_append": (C.c_int, [C.POINTER(PagedKv), C.POINTER(Ragged), C.POINTER(RopeAxes), C.c_void_p, C.c_int64,
+                                  C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int64,
+                                  C.c_void_p]),
+    "ti_op_paged_prefill": (C.c_int, [C.POINTER(PagedKv), C.POINTER(Ragged), C.POINTER(AttnForm), C.c_void_p,
+                                      C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p]),
+    "ti_op_paged_decode": (C.c_int, [C.POINTER(PagedKv), C.POINTER(Ragged), C.POINTER(AttnForm), C.c_void_p,
+                                     C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p]),
     "ti_op_transpose2d": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
     "ti_engine_create": (C.c_int, [C.POINTER(ModelDesc), C.POINTER(EngineOpts), C.POINTER(C.c_void_p)]),
     "ti_engine_destroy": (C.c_int, [C.c_void_p]),

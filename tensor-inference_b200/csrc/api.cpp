@@ -1,4 +1,5 @@
 // api.cpp — error state, device management and memory entry points of the C ABI.
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <string>
@@ -6,6 +7,8 @@
 #include "internal.h"
 
 namespace ti {
+
+cudaError_t pool_alloc(void** p, size_t bytes, int device, cudaStream_t s);
 
 static thread_local std::string g_last_error;
 
@@ -44,6 +47,23 @@ void rope_freqs(int head_dim, float theta, const ti_rope_scaling* sc, float* out
         }
         out[i] = f;
     }
+}
+
+// cudaMallocAsync from the device's default pool, whose release threshold the first
+// call raises: freed blocks stay in the pool across synchronisations (with the
+// default threshold of zero each first allocation after one maps memory anew, about
+// 400 us).  `device` is the current device.
+cudaError_t pool_alloc(void** p, size_t bytes, int device, cudaStream_t s) {
+    static std::atomic<bool> configured[64];
+    if (device >= 0 && device < 64 && !configured[device].load(std::memory_order_relaxed)) {
+        cudaMemPool_t pool;
+        if (cudaDeviceGetDefaultMemPool(&pool, device) == cudaSuccess) {
+            uint64_t thr = ~0ull;
+            cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &thr);
+        }
+        configured[device].store(true, std::memory_order_relaxed);
+    }
+    return cudaMallocAsync(p, bytes, s);
 }
 
 }  // namespace ti
@@ -127,17 +147,8 @@ ti_status ti_set_device(int device) {
 ti_status ti_malloc(int device, size_t bytes, void** ptr) {
     TI_CHECK(ptr, TI_ERR_INVALID, "ti_malloc: null out pointer");
     DeviceGuard g(device);
-    static bool configured[64] = {};
-    if (device >= 0 && device < 64 && !configured[device]) {
-        cudaMemPool_t pool;
-        if (cudaDeviceGetDefaultMemPool(&pool, device) == cudaSuccess) {
-            uint64_t thr = ~0ull;
-            cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &thr);
-        }
-        configured[device] = true;
-    }
     void* p = nullptr;
-    cudaError_t e = cudaMallocAsync(&p, bytes ? bytes : 1, (cudaStream_t)0);
+    cudaError_t e = pool_alloc(&p, bytes ? bytes : 1, device, (cudaStream_t)0);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return fail(TI_ERR_OOM, "ti_malloc(%zu): %s", bytes, cudaGetErrorString(e));

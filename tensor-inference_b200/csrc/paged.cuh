@@ -120,5 +120,21 @@ struct PagedAttn {
     int n_heads, n_kv, hd, dtype;
     int max_len;
 };
+// Pages as a 3-D tensor of 16-bit elements [hd/64][rows][64]: one box is the 16 rows of a page and
+// kv head in `parts` of their 64-dim parts, stored [part][16][64] with 128-byte swizzle.
+bool make_tmap_pages(CUtensorMap* m, const void* base, int rows, int hd, int parts);
+TI_DEVICE_INLINE void tma_load_page(void* dst, const CUtensorMap* map, int row, uint64_t* bar, int part = 0) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(0), "r"(row), "r"(part), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// stream-ordered memory of the device's pool, which keeps freed blocks for the next call (api.cpp)
+cudaError_t pool_alloc(void** p, size_t bytes, int device, cudaStream_t s);
+
+// both take their scratch from the pool; dev is the current device
+cudaError_t paged_decode_launch(const PagedAttn& p, int dev, cudaStream_t s);
 
 }  // namespace ti

@@ -80,6 +80,25 @@ cudaError_t paged_plain_launch(const PagedAttn& a, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+bool make_tmap_pages(CUtensorMap* m, const void* base, int rows, int hd, int parts) {
+    typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
+        return reinterpret_cast<EncodeFn>(e == cudaSuccess && q == cudaDriverEntryPointSuccess ? p : nullptr);
+    }();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)hd / 64};
+    const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, 128};
+    const cuuint32_t box[3] = {64, kPageTokens, (cuuint32_t)parts}, estr[3] = {1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 namespace {
 
 ti_status paged_args(const ti_paged_kv* kv, const ti_ragged* batch, const ti_attn_form* form, const void* q,
@@ -143,7 +162,7 @@ ti_status ti_op_paged_decode(const ti_paged_kv* kv, const ti_ragged* batch, cons
     int dev = 0;
     if (ti_status st = device_of(out, "paged_decode: out", &dev)) return st;
     DeviceGuard guard(dev);
-    TI_CUDA(paged_plain_launch(a, (cudaStream_t)stream));
+    TI_CUDA(paged_decode_launch(a, dev, (cudaStream_t)stream));
     return TI_OK;
 }
 

@@ -136,5 +136,6 @@ cudaError_t pool_alloc(void** p, size_t bytes, int device, cudaStream_t s);
 
 // both take their scratch from the pool; dev is the current device
 cudaError_t paged_decode_launch(const PagedAttn& p, int dev, cudaStream_t s);
+cudaError_t paged_prefill_launch(const PagedAttn& p, int dev, cudaStream_t s);
 
 }  // namespace ti

@@ -6,80 +6,6 @@
 
 namespace ti {
 
-// One warp per (token, head): a lane scores one key of 32 at a time, the warp keeps
-// one running maximum and sum, and each lane accumulates hd / 32 output dimensions.
-template <class T>
-__global__ void __launch_bounds__(128) k_paged_plain(const PagedAttn a) {
-    __shared__ float qs[4][256];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int t = blockIdx.x, h = blockIdx.y * 4 + warp;
-    const int hd = a.hd, nd = hd / 32;
-    if (h >= a.n_heads) return;
-    const int s = seq_of_token(a.r, t);
-    if (s >= a.r.n_seqs) return;
-    int t0, t1;
-    seq_tokens(a.r, s, t0, t1);
-    if (t < t0 || t >= t1) return;
-    const int kv_len = a.r.kv_len[s];
-    const int i = kv_len - (t1 - t0) + (t - t0);
-    const int32_t* row = table_row(a.r, s);
-    const int n_keys = row ? min(max(kv_len, 0), a.r.pt_stride * kPageTokens) : 0;
-    int lo, hi;
-    key_range(a.f, s, t, i, n_keys, lo, hi);
-    const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)t * a.q_stride + (int64_t)h * hd;
-    for (int d = lane; d < hd; d += 32) qs[warp][d] = Elem<T>::to_f(q[d]);
-    __syncwarp();
-    const int hk = h / (a.n_heads / a.n_kv);
-    const float slope = a.f.slopes ? a.f.slopes[h] : 0.f;
-    float m = -INFINITY, l = 0.f, o[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = 0.f;
-    for (int j0 = lo; j0 < hi; j0 += 32) {
-        const int j = j0 + lane;
-        const T* kr = nullptr;
-        const T* vr = nullptr;
-        float z = -INFINITY;
-        if (j < hi) {
-            const int page = row[j / kPageTokens];
-            const bool ok = page >= 0 && page < a.r.n_pages;
-            const int64_t off = (((int64_t)(ok ? page : 0) * a.n_kv + hk) * kPageTokens + j % kPageTokens) * hd;
-            kr = reinterpret_cast<const T*>(a.k_pages) + off;
-            vr = ok ? reinterpret_cast<const T*>(a.v_pages) + off : nullptr;
-            float acc = 0.f;
-            if (ok) for (int d = 0; d < hd; ++d) acc = fmaf(qs[warp][d], Elem<T>::to_f(kr[d]), acc);
-            z = acc * a.f.scale;
-            if (a.f.cap > 0.f) z = a.f.cap * tanhf(z / a.f.cap);
-            z -= slope * fabsf((float)(i - j));
-        }
-        const float mn = fmaxf(m, warp_max(z));
-        const float u = mn == -INFINITY ? 0.f : mn;
-        const float al = expf(m - u), p = j < hi ? expf(z - u) : 0.f;
-        m = mn;
-        l = l * al + warp_sum(p);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] *= al;
-        for (int k = 0; k < min(32, hi - j0); ++k) {
-            const float pk = __shfl_sync(0xffffffffu, p, k);
-            const T* vk = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, (unsigned long long)vr, k));
-            if (vk)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (e < nd) o[e] = fmaf(pk, Elem<T>::to_f(vk[lane + 32 * e]), o[e]);
-        }
-    }
-    T* out = reinterpret_cast<T*>(a.out) + (int64_t)t * a.out_stride + (int64_t)h * hd;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e < nd) out[lane + 32 * e] = Elem<T>::from_f(l == 0.f ? 0.f : o[e] / l);
-}
-
-cudaError_t paged_plain_launch(const PagedAttn& a, cudaStream_t s) {
-    const dim3 grid(a.r.n_tokens, (a.n_heads + 3) / 4);
-    if (a.dtype == TI_DTYPE_BF16) k_paged_plain<__nv_bfloat16><<<grid, 128, 0, s>>>(a);
-    else k_paged_plain<__half><<<grid, 128, 0, s>>>(a);
-    return cudaGetLastError();
-}
-
 bool make_tmap_pages(CUtensorMap* m, const void* base, int rows, int hd, int parts) {
     typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -149,7 +75,7 @@ ti_status ti_op_paged_prefill(const ti_paged_kv* kv, const ti_ragged* batch, con
     int dev = 0;
     if (ti_status st = device_of(out, "paged_prefill: out", &dev)) return st;
     DeviceGuard guard(dev);
-    TI_CUDA(paged_plain_launch(a, (cudaStream_t)stream));
+    TI_CUDA(paged_prefill_launch(a, dev, (cudaStream_t)stream));
     return TI_OK;
 }
 

@@ -1,0 +1,613 @@
+// paged_prefill.cu — attention of a ragged batch of new tokens over the paged cache (tcgen05).
+//
+// For the row (token, head) at position i: o = sum_j p_j v_j / sum_j p_j over the keys
+// [lo, hi) that it sees, p_j = 2^(z_j - m), z_j = log2(e) (cap tanh(q.k_j scale / cap) - slope |i - j|),
+// in one pass over key tiles with a running maximum m and sum per row.
+//
+// Rows: a tile holds 128 consecutive (token, head of the kv head's group) rows of one sequence, so
+// few tokens of a large group still fill the tensor cores, and K and V are shared by the group.
+// A CTA takes 256 rows (two tiles, "streams") at head_dim 64 and 128: while the tensor
+// cores work for one stream, the other's softmax runs.  At head_dim 256 the two outputs would not fit
+// in TMEM beside the scores: one stream of 128 rows with two score buffers.
+//
+// Warps: 0-3 and 4-7 softmax, one thread a row (stream 0, stream 1); 8 and 9 load K and V; 10 and 11
+// issue the MMAs of stream 0 and 1 (at head_dim 256 only warps 0-3 and 10).
+//   S = Q K^T       A = Q, B = K, both from shared memory (K-major, 128-byte swizzle)
+//   O += P V        A = P from TMEM (16-bit, over the scores it came from), B = V from shared memory
+//                   (N-major: a V row is 64 dims of one key)
+// K and V tiles are assembled from pages by TMA, a 2 KB box per page and 64 dims.
+// The output stays in TMEM; it is rescaled only when a row's maximum has grown by more than
+// 2^8 since the last time (P then stays under 2^8, far from overflow in either type), which
+// is rare after the first tiles.  P is rounded once to the operand type, half a step of
+// it (2^-9 of p at most for bf16) on each term, as the product's inputs must be; the
+// sum of p is taken before that rounding.
+//
+// Few rows over a long cache: the key tiles of a row tile are divided over gridDim.z CTAs,
+// whose partial (max, sum, output) rows k_prefill_join adds in order.
+//
+// Every wait is bounded; one that gives up stops all roles, the MMAs issued are waited for, and TMEM is freed.
+#include <algorithm>
+
+#include "paged.cuh"
+#include "tcgen05.cuh"
+
+namespace ti {
+
+constexpr int kPreThreads = 384;
+
+template <int HD>
+struct PreCfg {
+    static constexpr int NQ = HD <= 128 ? 2 : 1;    // row tiles (streams) of a CTA
+    static constexpr int ROWS = NQ * 128;
+    static constexpr int BN = HD <= 128 ? 128 : 64;  // keys of a tile
+    static constexpr int NB = 2;                    // score buffers: one a stream, or two for the one stream
+    static constexpr int NS = HD == 64 ? 4 : 2;     // K stages, and V stages
+    static constexpr int PARTS = HD / 64;
+    static constexpr int PAGES = BN / kPageTokens;
+    static constexpr uint32_t QBYTES = 128u * HD * 2;  // one row tile of Q
+    static constexpr uint32_t KBYTES = (uint32_t)BN * HD * 2;
+    static constexpr uint32_t S_COL = 0;            // score buffer b at b * BN, P over its first half
+    static constexpr uint32_t O_COL = 256;          // output of stream s at O_COL + s * HD
+    static_assert(NB * BN <= (int)O_COL && (int)O_COL + NQ * HD <= 512, "TMEM columns");
+};
+
+struct PreSmem {
+    uint32_t q, k, v, bar, misc, total;
+};
+template <int HD>
+__host__ __device__ constexpr PreSmem pre_smem() {
+    using C = PreCfg<HD>;
+    PreSmem L{};
+    uint32_t o = 0;
+    L.q = o;  // [streams][HD/64][128][64], 128-byte swizzle
+    o += C::NQ * C::QBYTES;
+    L.k = o;  // [stages][HD/64][BN][64]
+    o += C::NS * C::KBYTES;
+    L.v = o;
+    o += C::NS * C::KBYTES;
+    L.bar = o;  // k_full, k_empty, v_full, v_empty [NS]; v_edge, q_full; s_full, p_full [2]; pv, o_full [2]
+    o += 8 * (4 * C::NS + 2 + 8);
+    L.misc = o;  // [0] TMEM base, [1] stop, [2..3] lo, hi
+    o += 32;
+    L.total = o + 1024;
+    return L;
+}
+
+struct PreArgs {
+    PagedAttn p;
+    int group;
+    int cache_rows;
+    int vec;        // q and out rows are 16-byte aligned
+    int splits;
+    float* part_o;  // [splits][n_tokens][n_heads][hd]
+    float* part_ml;
+};
+
+// Which rows CTA x takes: tiles of ROWS rows, sequence after sequence, handed out from the last one
+// (the longest, under a causal mask) to the first.  seq < 0: no such tile.  Whole warps call it.
+struct RowTile {
+    int seq, row0;  // first row of the tile among the sequence's new tokens x group rows
+    int t0, t1;     // the sequence's tokens
+};
+template <int ROWS>
+TI_DEVICE_INLINE RowTile find_rows(const PreArgs& a, int x) {
+    const int lane = threadIdx.x & 31, n = a.p.r.n_seqs;
+    RowTile r{-1, 0, 0, 0};
+    auto tiles_of = [&](int s) {
+        int t0 = 0, t1 = 0;
+        if (s < n) seq_tokens(a.p.r, s, t0, t1);
+        return ((t1 - t0) * a.group + ROWS - 1) / ROWS;
+    };
+    int total = 0;
+    for (int base = 0; base < n; base += 32) total += tiles_of(base + lane);
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int want = total - 1 - x;
+    if (want < 0) return r;
+    int run = 0;
+    for (int base = 0; base < n; base += 32) {
+        const int c = tiles_of(base + lane);
+        int inc = c;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, want >= run + inc - c && want < run + inc);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            r.seq = base + l;
+            r.row0 = (want - (run + __shfl_sync(0xffffffffu, inc - c, l))) * ROWS;
+            seq_tokens(a.p.r, r.seq, r.t0, r.t1);
+            return r;
+        }
+        run += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return r;
+}
+
+// descriptor of V as the N-major B operand: rows of 64 dims (128 bytes, swizzled) per key, 8 keys
+// 1024 bytes apart (SBO), the next 64 dims a whole part of the tile apart (LBO)
+TI_DEVICE_INLINE uint64_t v_desc(uint32_t addr, uint32_t part_bytes) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(part_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// kind::f16, D fp32, A and B of one 16-bit type, M = 128, N = n; B N-major for P V
+template <class T>
+__host__ __device__ constexpr uint32_t pre_idesc(int n, bool b_nmajor) {
+    return (1u << 4) | (Elem<T>::kUmmaFmt << 7) | (Elem<T>::kUmmaFmt << 10) | (b_nmajor ? 1u << 16 : 0u) |
+           ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+template <int HD, class T, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kPreThreads, 1)
+    k_paged_prefill(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                    const __grid_constant__ PreArgs a) {
+    using C = PreCfg<HD>;
+    constexpr int BN = C::BN, NS = C::NS, NQ = C::NQ;
+    constexpr PreSmem L = pre_smem<HD>();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L.bar);
+    uint64_t* k_empty = k_full + NS;
+    uint64_t* v_full = k_empty + NS;
+    uint64_t* v_empty = v_full + NS;
+    uint64_t* v_edge = v_empty + NS;
+    uint64_t* q_full = v_edge + 1;
+    uint64_t* s_full = q_full + 1;
+    uint64_t* p_full = s_full + 2;
+    uint64_t* pv_done = p_full + 2;
+    uint64_t* o_full = pv_done + 2;
+    volatile int* misc = reinterpret_cast<volatile int*>(smem + L.misc);
+    int* range = reinterpret_cast<int*>(smem + L.misc) + 2;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int hk = blockIdx.y;
+
+    const RowTile rt = find_rows<C::ROWS>(a, blockIdx.x);
+    if (rt.seq < 0) return;  // the whole block
+    const int s = rt.seq;
+    const int n_rows = (rt.t1 - rt.t0) * a.group - rt.row0;  // rows of the sequence from the tile's first on
+
+    // ---- this thread's row (softmax threads): token, head, position, keys [lo, hi)
+    const int kv_len = a.p.r.kv_len[s];
+    const int32_t* table = table_row(a.p.r, s);
+    const int n_keys = table ? min(max(kv_len, 0), a.p.r.pt_stride * kPageTokens) : 0;
+    int token = 0, head = 0, pos = 0, lo = 0, hi = 0;
+    const bool mine = tid < C::ROWS && tid < n_rows;
+    if (mine) {
+        const int r = rt.row0 + tid;
+        token = rt.t0 + r / a.group;
+        head = hk * a.group + r % a.group;
+        pos = kv_len - (rt.t1 - token);
+        key_range(a.p.f, s, token, pos, n_keys, lo, hi);
+    }
+    if (tid == 0) {
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_empty[i], NQ);  // a commit from every stream
+            mbar_init(&v_full[i], 1);
+            mbar_init(&v_empty[i], NQ);
+        }
+        mbar_init(v_edge, 1);
+        mbar_init(q_full, 4 * NQ);  // the softmax warps
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);  // the warps of a stream
+            mbar_init(&pv_done[i], 1);
+            mbar_init(&o_full[i], 1);
+        }
+        misc[1] = 0;
+        range[0] = INT32_MAX;
+        range[1] = 0;
+        fence_barrier_init();
+    }
+    if (warp == 10) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)misc)),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    __syncthreads();
+    if (mine && hi > lo) {
+        atomicMin(&range[0], lo);
+        atomicMax(&range[1], hi);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = (uint32_t)misc[0];
+    const int key_lo = range[0], key_hi = range[1];  // keys some row of the CTA sees
+    int j0 = key_hi > key_lo ? key_lo / BN : 0, j1 = key_hi > key_lo ? (key_hi + BN - 1) / BN : 0;
+    if (a.splits > 1) {
+        const int per = (j1 - j0 + a.splits - 1) / a.splits;
+        j0 = min(j1, j0 + (int)blockIdx.z * per);
+        j1 = min(j1, j0 + per);
+    }
+    const int nt = j1 - j0;  // key tiles of this CTA
+
+    if (warp == 8) {
+        // ---------------------------------------------------------- K
+        for (int it = 0; it < nt; ++it) {
+            const int st = it % NS;
+            const int page = (j0 + it) * C::PAGES + lane;
+            const int id = lane < C::PAGES && page * kPageTokens < n_keys ? table[page] : -1;
+            const int row = id >= 0 && id < a.p.r.n_pages ? (id * a.p.n_kv + hk) * kPageTokens : a.cache_rows;
+            if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&k_empty[st], ((it / NS) & 1) ^ 1, nullptr, 0))) {
+                misc[1] = 1;
+                break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(&k_full[st], C::KBYTES);
+            __syncwarp();
+            if (lane < C::PAGES)
+#pragma unroll
+                for (int p = 0; p < C::PARTS; ++p)
+                    tma_load_page(smem + L.k + (uint32_t)st * C::KBYTES + (uint32_t)(p * BN + lane * kPageTokens) * 128u, &tk,
+                                  row, &k_full[st], p);
+            __syncwarp();
+        }
+        if (misc[1])  // a wait gave up: copies in flight land before the block ends
+            for (int i = 0; i < NS; ++i) mbar_wait_for(&k_full[i], 0, nullptr, 0, 1000000);
+    } else if (warp == 9) {
+        // ---------------------------------------------------------- V
+        int edges = 0;
+        for (int it = 0; it < nt; ++it) {
+            const int st = it % NS, k0 = (j0 + it) * BN;
+            const int page = (j0 + it) * C::PAGES + lane;
+            const int id = lane < C::PAGES && page * kPageTokens < n_keys ? table[page] : -1;
+            const int row = id >= 0 && id < a.p.r.n_pages ? (id * a.p.n_kv + hk) * kPageTokens : a.cache_rows;
+            if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&v_empty[st], ((it / NS) & 1) ^ 1, nullptr, 0))) {
+                misc[1] = 1;
+                break;
+            }
+            // a tile with keys that no row sees: those rows of V must be finite (their
+            // probabilities are zero), so they are zeroed before the MMAs may read the tile
+            const bool edge = k0 < key_lo || k0 + BN > key_hi;
+            uint64_t* bar = edge ? v_edge : &v_full[st];
+            uint8_t* vt = smem + L.v + (uint32_t)st * C::KBYTES;
+            if (lane == 0) mbar_arrive_expect_tx(bar, C::KBYTES);
+            __syncwarp();
+            if (lane < C::PAGES)
+#pragma unroll
+                for (int p = 0; p < C::PARTS; ++p)
+                    tma_load_page(vt + (uint32_t)(p * BN + lane * kPageTokens) * 128u, &tv, row, bar, p);
+            __syncwarp();
+            if (edge) {
+                if (__any_sync(0xffffffffu, !mbar_wait(v_edge, edges & 1, nullptr, 0))) {
+                    misc[1] = 1;
+                    break;
+                }
+                ++edges;
+                for (int c = lane; c < BN * C::PARTS * 8; c += 32) {
+                    const int r = (c >> 3) % BN;
+                    if (k0 + r < key_lo || k0 + r >= key_hi)
+                        *reinterpret_cast<uint4*>(vt + (uint32_t)c * 16u) = make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[st]);
+            }
+        }
+        if (misc[1])
+            for (int i = 0; i < NS; ++i) mbar_wait_for(&v_full[i], 0, nullptr, 0, 1000000);
+    } else if (warp >= 10) {
+        // ---------------------------------------------------------- MMA issue of one stream
+        const int q = warp - 10;
+        if (q < NQ && lane == 0 && nt > 0) {
+            const uint32_t id_s = pre_idesc<T>(BN, false), id_o = pre_idesc<T>(HD, true);
+            const uint64_t q_d = smem_desc_sw128(smem_u32(smem + L.q + (uint32_t)q * C::QBYTES));
+            const uint32_t o_t = tmem + C::O_COL + (uint32_t)(q * HD);
+            bool ok = true, issued = false;
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                if (ok && (misc[1] || !mbar_wait(bar, parity, nullptr, 0))) {
+                    misc[1] = 1;
+                    ok = false;
+                }
+                return ok;
+            };
+            auto scores = [&](int it) {  // S(it) = Q K(it)^T
+                const int st = it % NS, b = NQ == 2 ? q : it & 1;
+                if (!wait(&k_full[st], (it / NS) & 1)) return;
+                tc_fence_after();
+                const uint64_t k_d = smem_desc_sw128(smem_u32(smem + L.k + (uint32_t)st * C::KBYTES));
+#pragma unroll
+                for (int m = 0; m < HD / 16; ++m) {
+                    const uint32_t part = m >> 2, k = (m & 3) * 32;
+                    tc_mma(tmem + C::S_COL + (uint32_t)(b * BN), q_d + ((part * 128u * 128u + k) >> 4),
+                           k_d + ((part * (uint32_t)BN * 128u + k) >> 4), id_s, m > 0);
+                }
+                issued = true;
+                tc_commit(&k_empty[st]);
+                tc_commit(&s_full[b]);
+            };
+            auto values = [&](int it) {  // O += P(it) V(it)
+                const int st = it % NS, b = NQ == 2 ? q : it & 1;
+                const uint32_t n = NQ == 2 ? it : it >> 1;  // how often the buffer was used before
+                if (!wait(&p_full[b], n & 1) || !wait(&v_full[st], (it / NS) & 1)) return;
+                tc_fence_after();
+                const uint32_t p_t = tmem + C::S_COL + (uint32_t)(b * BN);
+                const uint64_t v_d = v_desc(smem_u32(smem + L.v + (uint32_t)st * C::KBYTES), (uint32_t)BN * 128u);
+#pragma unroll
+                for (int m = 0; m < BN / 16; ++m)
+                    tc_mma_ts(o_t, p_t + (uint32_t)(m * 8), v_d + ((m * 16u * 128u) >> 4), id_o, it > 0 || m > 0);
+                tc_commit(&v_empty[st]);
+                if (NQ == 1) tc_commit(&pv_done[0]);
+            };
+            wait(q_full, 0);
+            tc_fence_after();
+            if (ok) scores(0);
+            for (int it = 0; it < nt && ok; ++it) {
+                if (NQ == 1 && it + 1 < nt) scores(it + 1);  // into the other buffer, while softmax works
+                if (ok) values(it);
+                // the scores of the next tile overwrite P: issued after the product that reads it
+                if (NQ == 2 && ok && it + 1 < nt) scores(it + 1);
+            }
+            if (issued) {
+                tc_commit(&o_full[q]);
+                mbar_wait(&o_full[q], 0, nullptr, 0);  // every MMA retired before TMEM goes
+            }
+        }
+    } else if (warp < 4 * NQ) {
+        // ---------------------------------------------------------- softmax: one thread a row
+        const int q = warp >> 2;
+        const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        // ---- Q rows into shared memory (rows past the end are zero)
+        {
+            const T* src = reinterpret_cast<const T*>(a.p.q) + (mine ? (int64_t)token * a.p.q_stride + (int64_t)head * HD : 0);
+            uint8_t* qt = smem + L.q + (uint32_t)q * C::QBYTES;
+            constexpr int CH = HD / 8;        // 16-byte chunks of a row
+            constexpr int RP = 32 / (CH < 32 ? CH : 32);  // rows at a time
+            const int rl = lane / CH, c = lane % CH;
+            for (int i = 0; i < 32; i += RP) {
+                const T* p = reinterpret_cast<const T*>(
+                    __shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, i + rl));
+                const bool have = __shfl_sync(0xffffffffu, (int)mine, i + rl);
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (have) {
+                    if (a.vec) v = *reinterpret_cast<const uint4*>(p + c * 8);
+                    else {
+                        unsigned short* e = reinterpret_cast<unsigned short*>(&v);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) e[k] = reinterpret_cast<const unsigned short*>(p)[c * 8 + k];
+                    }
+                }
+                const int row = (warp & 3) * 32 + i + rl;
+                *reinterpret_cast<uint4*>(qt + (uint32_t)((c >> 3) * 128 + row) * 128u + (uint32_t)(((c & 7) ^ (row & 7)) << 4)) = v;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        const float scale2 = a.p.f.scale * kLog2E;
+        const float cap2 = a.p.f.cap * kLog2E;
+        const float c_in = CAP ? 2.f * kLog2E * a.p.f.scale / a.p.f.cap : 0.f;  // e^(2u) = 2^(c_in s)
+        const float slope2 = BIAS && mine ? a.p.f.slopes[head] * kLog2E : 0.f;
+        if (!mine) {  // rows past the end see everything: they must not force the masked path
+            lo = 0;
+            hi = INT32_MAX;
+        }
+        float m = -INFINITY, l = 0.f;
+        for (int it = 0; it < nt; ++it) {
+            const int b = NQ == 2 ? q : it & 1;
+            const uint32_t n = NQ == 2 ? it : it >> 1;
+            const int k0 = (j0 + it) * BN;
+            if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&s_full[b], n & 1, nullptr, 0))) {
+                misc[1] = 1;
+                break;
+            }
+            tc_fence_after();
+            float x[BN];
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) tmem_ld32_async(t_lane + C::S_COL + (uint32_t)(b * BN + c), x + c);
+            tmem_ld_done<BN>(x);
+            if constexpr (CAP) {
+                // cap tanh(u) = cap - 2 cap / (e^(2u) + 1)
+#pragma unroll
+                for (int c = 0; c < BN; ++c) x[c] = fmaf(-2.f * cap2, __frcp_rn(ex2(x[c] * c_in) + 1.f), cap2);
+            } else {
+#pragma unroll
+                for (int c = 0; c < BN; ++c) x[c] *= scale2;
+            }
+            if constexpr (BIAS) {
+                const float d0 = (float)(pos - k0);
+#pragma unroll
+                for (int c = 0; c < BN; ++c) x[c] = fmaf(-slope2, fabsf(d0 - (float)c), x[c]);
+            }
+            if (!__all_sync(0xffffffffu, lo <= k0 && hi >= k0 + BN)) {
+                const int cl = lo - k0, ch = hi - k0;
+#pragma unroll
+                for (int c = 0; c < BN; ++c) x[c] = c >= cl && c < ch ? x[c] : -INFINITY;
+            }
+            float mx = x[0];
+#pragma unroll
+            for (int c = 1; c < BN; ++c) mx = fmaxf(mx, x[c]);
+            // ---- lazily rescaled maximum
+            bool grow = mx > m + 8.f;  // (m = -inf: the first keys of the row)
+            if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
+                if (NQ == 1 && it > 0) {  // with two streams s_full(it) already says that P V (it - 1) is done
+                    if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&pv_done[0], (it - 1) & 1, nullptr, 0))) {
+                        misc[1] = 1;
+                        break;
+                    }
+                    tc_fence_after();
+                }
+                const float f = grow ? ex2(m - mx) : 1.f;
+                l *= f;
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    float o[32];
+                    const uint32_t at = t_lane + C::O_COL + (uint32_t)(q * HD + c);
+                    uint32_t w[32];
+                    tmem_ld32(at, o);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * f);
+                    tmem_st32(at, w);
+                }
+            }
+            if (grow) m = mx;
+            const float u = m == -INFINITY ? 0.f : m;
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int h = 0; h < BN; h += 64) {
+                uint32_t w[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                    const float p0 = ex2(x[h + 2 * c] - u), p1 = ex2(x[h + 2 * c + 1] - u);
+                    s0 += p0;
+                    s1 += p1;
+                    w[c] = Elem<T>::pack(p0, p1);
+                }
+                tmem_st32(t_lane + C::S_COL + (uint32_t)(b * BN + h / 2), w);
+            }
+            l += s0 + s1;
+            tmem_st_done();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[b]);
+        }
+        // ---- output rows
+        bool good = true;
+        if (nt > 0) {
+            good = !__any_sync(0xffffffffu, misc[1] || !mbar_wait(&o_full[q], 0, nullptr, 0));
+            tc_fence_after();
+        }
+        if (a.splits > 1) {
+            const int64_t row = ((int64_t)blockIdx.z * a.p.r.n_tokens + token) * a.p.n_heads + head;
+            if (mine) reinterpret_cast<float2*>(a.part_ml)[row] = nt > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+            if (nt > 0 && good) {
+                for (int c = 0; c < HD; c += 32) {
+                    float o[32];
+                    tmem_ld32(t_lane + C::O_COL + (uint32_t)(q * HD + c), o);
+                    if (mine)
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            *reinterpret_cast<float4*>(a.part_o + row * HD + c + k) =
+                                make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                }
+            }
+        } else {
+            T* dst = reinterpret_cast<T*>(a.p.out) + (int64_t)token * a.p.out_stride + (int64_t)head * HD;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            for (int c = 0; c < HD; c += 32) {
+                float o[32];
+                if (nt > 0) tmem_ld32(t_lane + C::O_COL + (uint32_t)(q * HD + c), o);
+                uint32_t w[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    w[k] = nt > 0 && l != 0.f ? Elem<T>::pack(o[2 * k] * inv, o[2 * k + 1] * inv) : 0u;
+                if (mine) {
+                    if (a.vec) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            *reinterpret_cast<uint4*>(dst + c + k * 8) =
+                                make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                    } else {
+                        unsigned short* e = reinterpret_cast<unsigned short*>(dst + c);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            e[2 * k] = (unsigned short)(w[k] & 0xffffu);
+                            e[2 * k + 1] = (unsigned short)(w[k] >> 16);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 10) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// One warp a row: the partials of a row whose keys were divided, in order.
+template <class T>
+__global__ void __launch_bounds__(128) k_prefill_join(const __grid_constant__ PreArgs a) {
+    const int lane = threadIdx.x & 31, HD = a.p.hd;
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    pdl_wait();
+    const int64_t rows = (int64_t)a.p.r.n_tokens * a.p.n_heads;
+    if (r >= rows) return;
+    const int t = (int)(r / a.p.n_heads), h = (int)(r % a.p.n_heads);
+    if (seq_of_token(a.p.r, t) >= a.p.r.n_seqs || (a.p.r.start && t < a.p.r.start[0])) return;  // nobody's token
+    float M = -INFINITY;
+    for (int z = 0; z < a.splits; ++z) M = fmaxf(M, a.part_ml[(z * rows + r) * 2]);
+    const float u = M == -INFINITY ? 0.f : M;
+    T* out = reinterpret_cast<T*>(a.p.out) + (int64_t)t * a.p.out_stride + (int64_t)h * HD;
+    for (int d = lane * 2; d < HD; d += 64) {
+        float l = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll 4
+        for (int z = 0; z < a.splits; ++z) {
+            const float2 x = *reinterpret_cast<const float2*>(a.part_ml + (z * rows + r) * 2);
+            if (x.x == -INFINITY && x.y == 0.f) continue;  // saw nothing: its output was not written
+            const float2 v = *reinterpret_cast<const float2*>(a.part_o + (z * rows + r) * HD + d);
+            const float f = ex2(x.x - u);
+            l = fmaf(x.y, f, l);
+            o0 = fmaf(v.x, f, o0);
+            o1 = fmaf(v.y, f, o1);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        out[d] = Elem<T>::from_f(o0 * inv);
+        out[d + 1] = Elem<T>::from_f(o1 * inv);
+    }
+}
+
+namespace {
+
+template <int HD, class T>
+const void* pre_func(bool cap, bool bias) {
+    if (cap) return bias ? (const void*)&k_paged_prefill<HD, T, true, true> : (const void*)&k_paged_prefill<HD, T, true, false>;
+    return bias ? (const void*)&k_paged_prefill<HD, T, false, true> : (const void*)&k_paged_prefill<HD, T, false, false>;
+}
+template <class T>
+const void* pre_func(int hd, bool cap, bool bias) {
+    return hd == 64 ? pre_func<64, T>(cap, bias) : hd == 128 ? pre_func<128, T>(cap, bias) : pre_func<256, T>(cap, bias);
+}
+
+}  // namespace
+
+cudaError_t paged_prefill_launch(const PagedAttn& p, int dev, cudaStream_t s) {
+    const int sms = num_sms(dev);
+    PreArgs a{};
+    a.p = p;
+    a.group = p.n_heads / p.n_kv;
+    a.cache_rows = p.r.n_pages * p.n_kv * kPageTokens;
+    a.vec = (((uintptr_t)p.q | (uintptr_t)p.out) & 15) == 0 && p.q_stride % 8 == 0 && p.out_stride % 8 == 0;
+    const int rows = p.hd <= 128 ? 256 : 128, bn = p.hd <= 128 ? 128 : 64;
+    // every sequence may end in a part of a tile; CTAs past the last tile return at once
+    const int64_t tiles = (int64_t)p.r.n_tokens * a.group / rows + std::min(p.r.n_seqs, p.r.n_tokens);
+    if (tiles > INT32_MAX) return cudaErrorInvalidValue;
+    // key tiles are divided when the row tiles alone leave SMs idle, down to four tiles a CTA
+    const int64_t span = p.f.window > 0 ? std::min<int64_t>(p.max_len, (int64_t)p.f.window + rows) : p.max_len;
+    const int64_t ctas = tiles * p.n_kv, key_tiles = (span + bn - 1) / bn;
+    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({sms / ctas, key_tiles / 4, 64}));
+    CUtensorMap tk, tv;
+    if (!make_tmap_pages(&tk, p.k_pages, a.cache_rows, p.hd, 1) || !make_tmap_pages(&tv, p.v_pages, a.cache_rows, p.hd, 1))
+        return cudaErrorInvalidValue;
+    const bool bf = p.dtype == TI_DTYPE_BF16, cap = p.f.cap > 0.f, bias = p.f.slopes != nullptr;
+    const void* f = bf ? pre_func<__nv_bfloat16>(p.hd, cap, bias) : pre_func<__half>(p.hd, cap, bias);
+    const size_t smem = p.hd == 64 ? pre_smem<64>().total : p.hd == 128 ? pre_smem<128>().total : pre_smem<256>().total;
+    cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    float* scratch = nullptr;
+    const size_t n = (size_t)a.splits * p.r.n_tokens * p.n_heads;
+    if (a.splits > 1) {
+        e = pool_alloc(reinterpret_cast<void**>(&scratch), n * (p.hd + 2) * sizeof(float), dev, s);
+        if (e != cudaSuccess) return e;
+        a.part_o = scratch;
+        a.part_ml = scratch + n * p.hd;
+    }
+    void* args[] = {&tk, &tv, &a};
+    e = launch_pdl(f, dim3((unsigned)tiles, p.n_kv, a.splits), dim3(kPreThreads), smem, s, args, false);
+    if (a.splits > 1) {
+        if (e == cudaSuccess) {
+            void* jargs[] = {&a};
+            const void* j = bf ? (const void*)&k_prefill_join<__nv_bfloat16> : (const void*)&k_prefill_join<__half>;
+            const int64_t rows_all = (int64_t)p.r.n_tokens * p.n_heads;
+            e = launch_pdl(j, dim3((unsigned)((rows_all + 3) / 4)), dim3(128), 0, s, jargs, true);
+        }
+        const cudaError_t g = cudaFreeAsync(scratch, s);
+        if (e == cudaSuccess) e = g;
+    }
+    return e;
+}
+
+}  // namespace ti

@@ -40,8 +40,8 @@ ti_status paged_args(const ti_paged_kv* kv, const ti_ragged* batch, const ti_att
              "%s: a stride is less than a token's %lld elements", who, (long long)width);
     ti_attn_form plain{};
     const ti_attn_form& f = form ? *form : plain;
-    TI_CHECK(std::isfinite(f.scale) && std::isfinite(f.softcap) && f.softcap >= 0.f, TI_ERR_INVALID,
-             "%s: scale and softcap must be finite, softcap not negative", who);
+    TI_CHECK(std::isfinite(f.scale) && std::isfinite(f.softcap) && f.scale >= 0.f && f.softcap >= 0.f, TI_ERR_INVALID,
+             "%s: scale and softcap must be finite and not negative", who);
     a->r = ragged_dev(kv, batch);
     a->f = FormDev{f.scale != 0.f ? f.scale : 1.0f / sqrtf((float)hd), f.softcap, f.slopes, f.sliding_window, f.prefix,
                    f.doc_start};

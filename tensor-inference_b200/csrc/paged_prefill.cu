@@ -34,6 +34,64 @@
 namespace ti {
 
 constexpr int kPreThreads = 384;
+// Registers: the block is launched with 168 a thread (384 x 168 = 64,512); with two streams the
+// loading and issuing warps hand theirs to the softmax warps, which hold a whole row of scores:
+// 128 x 56 + 256 x 224 = 64,512.
+constexpr int kRegsLaunch = 168, kRegsOther = 56, kRegsSoftmax = 224;
+static_assert(128 * kRegsOther + 256 * kRegsSoftmax == kPreThreads * kRegsLaunch, "the shares are what was launched");
+template <int N>
+TI_DEVICE_INLINE void regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+TI_DEVICE_INLINE void regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// packed pairs of fp32, each rounded to nearest
+TI_DEVICE_INLINE float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+          "l"(reinterpret_cast<unsigned long long&>(c)));
+    return d;
+}
+TI_DEVICE_INLINE float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+TI_DEVICE_INLINE float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
+TI_DEVICE_INLINE float2 dup2(float v) { return make_float2(v, v); }
+TI_DEVICE_INLINE float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+TI_DEVICE_INLINE float min3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+TI_DEVICE_INLINE float rcp_approx(float v) {
+    float d;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v));
+    return d;
+}
+
+// tanh(u) / u in z = u^2 for |u| <= 3/4: the polynomial of degree 4 whose largest error in tanh is smallest
+// (linear programming over 3,000 points), 2.1e-07
+constexpr float kTanhRange = 0.75f;
+constexpr float kTanh0 = 0.99999719858f, kTanh1 = -0.3332307636f, kTanh2 = 0.13226091861f, kTanh3 = -0.0492804534f, kTanh4 = 0.01231883652f;
 
 template <int HD>
 struct PreCfg {
@@ -158,7 +216,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     uint64_t* o_full = pv_done + 2;
     volatile int* misc = reinterpret_cast<volatile int*>(smem + L.misc);
     int* range = reinterpret_cast<int*>(smem + L.misc) + 2;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform, and known to be
     const int hk = blockIdx.y;
 
     const RowTile rt = find_rows<C::ROWS>(a, blockIdx.x);
@@ -213,7 +272,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = (uint32_t)misc[0];
+    const uint32_t tmem = __shfl_sync(0xffffffffu, (uint32_t)misc[0], 0);
     const int key_lo = range[0], key_hi = range[1];  // keys some row of the CTA sees
     int j0 = key_hi > key_lo ? key_lo / BN : 0, j1 = key_hi > key_lo ? (key_hi + BN - 1) / BN : 0;
     if (a.splits > 1) {
@@ -221,8 +280,23 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         j0 = min(j1, j0 + (int)blockIdx.z * per);
         j1 = min(j1, j0 + per);
     }
-    const int nt = j1 - j0;  // key tiles of this CTA
+    const int nt = __shfl_sync(0xffffffffu, j1 - j0, 0);  // key tiles of this CTA
 
+    // a tile from its pages (lane l holds the pool row of page l), one lane issuing
+    auto load_tile = [&](uint8_t* dst, const CUtensorMap* map, int row, uint64_t* bar) {
+        const bool one = elect_one();
+        if (one) mbar_arrive_expect_tx(bar, C::KBYTES);
+#pragma unroll
+        for (int i = 0; i < C::PAGES; ++i) {
+            const int r = __shfl_sync(0xffffffffu, row, i);
+            if (one)
+#pragma unroll
+                for (int p = 0; p < C::PARTS; ++p)
+                    tma_load_page(dst + (uint32_t)(p * BN + i * kPageTokens) * 128u, map, r, bar, p);
+        }
+        __syncwarp();
+    };
+    if (NQ == 2 && warp >= 8) regs_dec<kRegsOther>();
     if (warp == 8) {
         // ---------------------------------------------------------- K
         for (int it = 0; it < nt; ++it) {
@@ -234,14 +308,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                 misc[1] = 1;
                 break;
             }
-            if (lane == 0) mbar_arrive_expect_tx(&k_full[st], C::KBYTES);
-            __syncwarp();
-            if (lane < C::PAGES)
-#pragma unroll
-                for (int p = 0; p < C::PARTS; ++p)
-                    tma_load_page(smem + L.k + (uint32_t)st * C::KBYTES + (uint32_t)(p * BN + lane * kPageTokens) * 128u, &tk,
-                                  row, &k_full[st], p);
-            __syncwarp();
+            load_tile(smem + L.k + (uint32_t)st * C::KBYTES, &tk, row, &k_full[st]);
         }
         if (misc[1])  // a wait gave up: copies in flight land before the block ends
             for (int i = 0; i < NS; ++i) mbar_wait_for(&k_full[i], 0, nullptr, 0, 1000000);
@@ -262,13 +329,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             const bool edge = k0 < key_lo || k0 + BN > key_hi;
             uint64_t* bar = edge ? v_edge : &v_full[st];
             uint8_t* vt = smem + L.v + (uint32_t)st * C::KBYTES;
-            if (lane == 0) mbar_arrive_expect_tx(bar, C::KBYTES);
-            __syncwarp();
-            if (lane < C::PAGES)
-#pragma unroll
-                for (int p = 0; p < C::PARTS; ++p)
-                    tma_load_page(vt + (uint32_t)(p * BN + lane * kPageTokens) * 128u, &tv, row, bar, p);
-            __syncwarp();
+            load_tile(vt, &tv, row, bar);
             if (edge) {
                 if (__any_sync(0xffffffffu, !mbar_wait(v_edge, edges & 1, nullptr, 0))) {
                     misc[1] = 1;
@@ -290,13 +351,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     } else if (warp >= 10) {
         // ---------------------------------------------------------- MMA issue of one stream
         const int q = warp - 10;
-        if (q < NQ && lane == 0 && nt > 0) {
+        if (q < NQ && nt > 0) {
             const uint32_t id_s = pre_idesc<T>(BN, false), id_o = pre_idesc<T>(HD, true);
             const uint64_t q_d = smem_desc_sw128(smem_u32(smem + L.q + (uint32_t)q * C::QBYTES));
             const uint32_t o_t = tmem + C::O_COL + (uint32_t)(q * HD);
+            const bool one = elect_one();
             bool ok = true, issued = false;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
-                if (ok && (misc[1] || !mbar_wait(bar, parity, nullptr, 0))) {
+                if (ok && !__all_sync(0xffffffffu, !misc[1] && mbar_wait(bar, parity, nullptr, 0))) {
                     misc[1] = 1;
                     ok = false;
                 }
@@ -307,28 +369,34 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                 if (!wait(&k_full[st], (it / NS) & 1)) return;
                 tc_fence_after();
                 const uint64_t k_d = smem_desc_sw128(smem_u32(smem + L.k + (uint32_t)st * C::KBYTES));
+                if (one) {
 #pragma unroll
-                for (int m = 0; m < HD / 16; ++m) {
-                    const uint32_t part = m >> 2, k = (m & 3) * 32;
-                    tc_mma(tmem + C::S_COL + (uint32_t)(b * BN), q_d + ((part * 128u * 128u + k) >> 4),
-                           k_d + ((part * (uint32_t)BN * 128u + k) >> 4), id_s, m > 0);
+                    for (int m = 0; m < HD / 16; ++m) {
+                        const uint32_t part = m >> 2, k = (m & 3) * 32;
+                        tc_mma(tmem + C::S_COL + (uint32_t)(b * BN), q_d + ((part * 128u * 128u + k) >> 4),
+                               k_d + ((part * (uint32_t)BN * 128u + k) >> 4), id_s, m > 0);
+                    }
+                    tc_commit(&k_empty[st]);
+                    tc_commit(&s_full[b]);
                 }
+                __syncwarp();
                 issued = true;
-                tc_commit(&k_empty[st]);
-                tc_commit(&s_full[b]);
             };
             auto values = [&](int it) {  // O += P(it) V(it)
                 const int st = it % NS, b = NQ == 2 ? q : it & 1;
                 const uint32_t n = NQ == 2 ? it : it >> 1;  // how often the buffer was used before
-                if (!wait(&p_full[b], n & 1) || !wait(&v_full[st], (it / NS) & 1)) return;
+                if (!wait(&v_full[st], (it / NS) & 1) || !wait(&p_full[b], n & 1)) return;
                 tc_fence_after();
                 const uint32_t p_t = tmem + C::S_COL + (uint32_t)(b * BN);
                 const uint64_t v_d = v_desc(smem_u32(smem + L.v + (uint32_t)st * C::KBYTES), (uint32_t)BN * 128u);
+                if (one) {
 #pragma unroll
-                for (int m = 0; m < BN / 16; ++m)
-                    tc_mma_ts(o_t, p_t + (uint32_t)(m * 8), v_d + ((m * 16u * 128u) >> 4), id_o, it > 0 || m > 0);
-                tc_commit(&v_empty[st]);
-                if (NQ == 1) tc_commit(&pv_done[0]);
+                    for (int m = 0; m < BN / 16; ++m)
+                        tc_mma_ts(o_t, p_t + (uint32_t)(m * 8), v_d + ((m * 16u * 128u) >> 4), id_o, it > 0 || m > 0);
+                    tc_commit(&v_empty[st]);
+                    if (NQ == 1) tc_commit(&pv_done[0]);
+                }
+                __syncwarp();
             };
             wait(q_full, 0);
             tc_fence_after();
@@ -340,12 +408,14 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                 if (NQ == 2 && ok && it + 1 < nt) scores(it + 1);
             }
             if (issued) {
-                tc_commit(&o_full[q]);
+                if (one) tc_commit(&o_full[q]);
+                __syncwarp();
                 mbar_wait(&o_full[q], 0, nullptr, 0);  // every MMA retired before TMEM goes
             }
         }
     } else if (warp < 4 * NQ) {
         // ---------------------------------------------------------- softmax: one thread a row
+        if (NQ == 2) regs_inc<kRegsSoftmax>();
         const int q = warp >> 2;
         const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         // ---- Q rows into shared memory (rows past the end are zero)
@@ -375,9 +445,15 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
         }
+        // z (base 2) = mult x, where x is q.k itself when nothing else is done to the scores
+        const float mult = CAP || BIAS ? 1.f : a.p.f.scale * kLog2E;
         const float scale2 = a.p.f.scale * kLog2E;
+        const float u1 = CAP ? a.p.f.scale / a.p.f.cap : 0.f;  // u = u1 q.k
         const float cap2 = a.p.f.cap * kLog2E;
-        const float c_in = CAP ? 2.f * kLog2E * a.p.f.scale / a.p.f.cap : 0.f;  // e^(2u) = 2^(c_in s)
+        const float s_max = CAP ? kTanhRange / u1 : 0.f;       // |q.k| up to which the polynomial holds
+        // z = x (c0 + c1 x^2 + ...), x = q.k
+        const float c0 = cap2 * u1 * kTanh0, c1 = cap2 * u1 * u1 * u1 * kTanh1, c2 = c1 * u1 * u1 * (kTanh2 / kTanh1),
+                    c3 = c2 * u1 * u1 * (kTanh3 / kTanh2), c4 = c3 * u1 * u1 * (kTanh4 / kTanh3);
         const float slope2 = BIAS && mine ? a.p.f.slopes[head] * kLog2E : 0.f;
         if (!mine) {  // rows past the end see everything: they must not force the masked path
             lo = 0;
@@ -397,27 +473,79 @@ __global__ void __launch_bounds__(kPreThreads, 1)
 #pragma unroll
             for (int c = 0; c < BN; c += 32) tmem_ld32_async(t_lane + C::S_COL + (uint32_t)(b * BN + c), x + c);
             tmem_ld_done<BN>(x);
+            // a tile that some row of the warp sees in part
+            const bool edge = !__all_sync(0xffffffffu, lo <= k0 && hi >= k0 + BN);
+            auto row_max = [&] {
+                float m4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int c = 4; c < BN - 4; c += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) m4[k] = max3(m4[k], x[c + k], x[c + 4 + k]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], x[BN - 4 + k]);
+                return fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
+            };
+            auto poly = [&](float2 v, float2 add) {  // z of a pair + add
+                const float2 z = mul2(v, v);
+                float2 h = fma2(dup2(c4), z, dup2(c3));
+                h = fma2(h, z, dup2(c2));
+                h = fma2(h, z, dup2(c1));
+                h = fma2(h, z, dup2(c0));
+                return fma2(h, v, add);
+            };
+            bool small = false;  // capped scores within the polynomial's range
+            float mx;
             if constexpr (CAP) {
-                // cap tanh(u) = cap - 2 cap / (e^(2u) + 1)
+                mx = row_max();
+                float n4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int c = 0; c < BN; ++c) x[c] = fmaf(-2.f * cap2, __frcp_rn(ex2(x[c] * c_in) + 1.f), cap2);
-            } else {
+                for (int c = 4; c < BN - 4; c += 8)
 #pragma unroll
-                for (int c = 0; c < BN; ++c) x[c] *= scale2;
+                    for (int k = 0; k < 4; ++k) n4[k] = min3(n4[k], x[c + k], x[c + 4 + k]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) n4[k] = fminf(n4[k], x[BN - 4 + k]);
+                const float mn = fminf(min3(n4[0], n4[1], n4[2]), n4[3]);
+                // (max and min drop a NaN, and both ways give NaN for it)
+                small = !edge && __all_sync(0xffffffffu, mx <= s_max && mn >= -s_max);
+                if (small && !BIAS) {
+                    mx = poly(make_float2(mx, 0.f), dup2(0.f)).x;  // monotonic: the maximum of the capped scores
+                } else if (small) {
+#pragma unroll
+                    for (int c = 0; c < BN; c += 2) {
+                        const float2 y = poly(make_float2(x[c], x[c + 1]), dup2(0.f));
+                        x[c] = y.x;
+                        x[c + 1] = y.y;
+                    }
+                } else {
+                    // cap tanh(u) = cap - 2 cap / (e^(2u) + 1), whatever u is
+                    const float c_in = 2.f * kLog2E * u1;
+#pragma unroll
+                    for (int c = 0; c < BN; ++c) x[c] = fmaf(-2.f * cap2, rcp_approx(ex2(x[c] * c_in) + 1.f), cap2);
+                }
             }
             if constexpr (BIAS) {
                 const float d0 = (float)(pos - k0);
+                if (!edge && __all_sync(0xffffffffu, pos >= k0 + BN - 1 || !mine)) {
+                    // every key is at or before the row: -slope (i - j) is a line in j
+                    const float2 sl = dup2(slope2), sc = dup2(CAP ? 1.f : scale2);
+                    const float b0 = -slope2 * d0;
 #pragma unroll
-                for (int c = 0; c < BN; ++c) x[c] = fmaf(-slope2, fabsf(d0 - (float)c), x[c]);
+                    for (int c = 0; c < BN; c += 2) {
+                        const float2 y = fma2(make_float2(x[c], x[c + 1]), sc, fma2(sl, make_float2((float)c, (float)(c + 1)), dup2(b0)));
+                        x[c] = y.x;
+                        x[c + 1] = y.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < BN; ++c) x[c] = fmaf(-slope2, fabsf(d0 - (float)c), CAP ? x[c] : x[c] * scale2);
+                }
             }
-            if (!__all_sync(0xffffffffu, lo <= k0 && hi >= k0 + BN)) {
+            if (edge) {
                 const int cl = lo - k0, ch = hi - k0;
 #pragma unroll
                 for (int c = 0; c < BN; ++c) x[c] = c >= cl && c < ch ? x[c] : -INFINITY;
             }
-            float mx = x[0];
-#pragma unroll
-            for (int c = 1; c < BN; ++c) mx = fmaxf(mx, x[c]);
+            if (!CAP || BIAS || !small) mx = row_max() * mult;
             // ---- lazily rescaled maximum
             bool grow = mx > m + 8.f;  // (m = -inf: the first keys of the row)
             if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
@@ -443,20 +571,25 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             }
             if (grow) m = mx;
             const float u = m == -INFINITY ? 0.f : m;
-            float s0 = 0.f, s1 = 0.f;
+            float2 sum = dup2(0.f);
+            const float2 mu = dup2(-u), mm = dup2(mult);
+            auto exps = [&](auto&& arg) {
 #pragma unroll
-            for (int h = 0; h < BN; h += 64) {
-                uint32_t w[32];
+                for (int h = 0; h < BN; h += 64) {
+                    uint32_t w[32];
 #pragma unroll
-                for (int c = 0; c < 32; ++c) {
-                    const float p0 = ex2(x[h + 2 * c] - u), p1 = ex2(x[h + 2 * c + 1] - u);
-                    s0 += p0;
-                    s1 += p1;
-                    w[c] = Elem<T>::pack(p0, p1);
+                    for (int c = 0; c < 32; ++c) {
+                        const float2 y = arg(make_float2(x[h + 2 * c], x[h + 2 * c + 1]));
+                        const float2 p = make_float2(ex2(y.x), ex2(y.y));
+                        sum = add2(sum, p);
+                        w[c] = Elem<T>::pack(p.x, p.y);
+                    }
+                    tmem_st32(t_lane + C::S_COL + (uint32_t)(b * BN + h / 2), w);
                 }
-                tmem_st32(t_lane + C::S_COL + (uint32_t)(b * BN + h / 2), w);
-            }
-            l += s0 + s1;
+            };
+            if (CAP && !BIAS && small) exps([&](float2 v) { return poly(v, mu); });
+            else exps([&](float2 v) { return fma2(v, mm, mu); });
+            l += sum.x + sum.y;
             tmem_st_done();
             tc_fence_before();
             __syncwarp();

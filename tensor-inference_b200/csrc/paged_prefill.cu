@@ -10,8 +10,8 @@
 // cores work for one stream, the other's softmax runs.  At head_dim 256 the two outputs would not fit
 // in TMEM beside the scores: one stream of 128 rows with two score buffers.
 //
-// Warps: 0-3 and 4-7 softmax, one thread a row (stream 0, stream 1); 8 and 9 load K and V; 10 and 11
-// issue the MMAs of stream 0 and 1 (at head_dim 256 only warps 0-3 and 10).
+// Warps: 0-3 and 4-7 softmax, one thread a row (stream 0, stream 1; at head_dim 256 only 0-3); 8 and 9
+// load K and V; 10 issues the MMAs.
 //   S = Q K^T       A = Q, B = K, both from shared memory (K-major, 128-byte swizzle)
 //   O += P V        A = P from TMEM (16-bit, over the scores it came from), B = V from shared memory
 //                   (N-major: a V row is 64 dims of one key)
@@ -123,8 +123,8 @@ __host__ __device__ constexpr PreSmem pre_smem() {
     o += C::NS * C::KBYTES;
     L.v = o;
     o += C::NS * C::KBYTES;
-    L.bar = o;  // k_full, k_empty, v_full, v_empty [NS]; v_edge, q_full; s_full, p_full [2]; pv, o_full [2]
-    o += 8 * (4 * C::NS + 2 + 8);
+    L.bar = o;  // k_full, k_empty, v_full, v_empty [NS]; v_edge, q_full; s_full, p_full, pv_done, o_full [2]; mma_done
+    o += 8 * (4 * C::NS + 2 + 8 + 2);
     L.misc = o;  // [0] TMEM base, [1] stop, [2..3] lo, hi
     o += 32;
     L.total = o + 1024;
@@ -214,6 +214,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     uint64_t* p_full = s_full + 2;
     uint64_t* pv_done = p_full + 2;
     uint64_t* o_full = pv_done + 2;
+    uint64_t* mma_done = o_full + 2;
     volatile int* misc = reinterpret_cast<volatile int*>(smem + L.misc);
     int* range = reinterpret_cast<int*>(smem + L.misc) + 2;
     const int tid = threadIdx.x, lane = tid & 31;
@@ -241,11 +242,12 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
             mbar_init(&k_full[i], 1);
-            mbar_init(&k_empty[i], NQ);  // a commit from every stream
+            mbar_init(&k_empty[i], 1);
             mbar_init(&v_full[i], 1);
-            mbar_init(&v_empty[i], NQ);
+            mbar_init(&v_empty[i], 1);
         }
         mbar_init(v_edge, 1);
+        mbar_init(mma_done, 1);
         mbar_init(q_full, 4 * NQ);  // the softmax warps
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
@@ -349,12 +351,13 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         if (misc[1])
             for (int i = 0; i < NS; ++i) mbar_wait_for(&v_full[i], 0, nullptr, 0, 1000000);
     } else if (warp >= 10) {
-        // ---------------------------------------------------------- MMA issue of one stream
-        const int q = warp - 10;
-        if (q < NQ && nt > 0) {
+        // ---------------------------------------------------------- MMA issue
+        // One warp for both streams: a stream's P V and next scores are issued together, so the
+        // tensor cores finish one stream's batch while the other's softmax runs.  With a warp a stream
+        // the batches interleave, both streams wait for both, and then both softmaxes
+        // compete for the exponentials (4,800 against 3,500 cycles a pair of tiles).
+        if (warp == 10 && nt > 0) {
             const uint32_t id_s = pre_idesc<T>(BN, false), id_o = pre_idesc<T>(HD, true);
-            const uint64_t q_d = smem_desc_sw128(smem_u32(smem + L.q + (uint32_t)q * C::QBYTES));
-            const uint32_t o_t = tmem + C::O_COL + (uint32_t)(q * HD);
             const bool one = elect_one();
             bool ok = true, issued = false;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -364,10 +367,11 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                 }
                 return ok;
             };
-            auto scores = [&](int it) {  // S(it) = Q K(it)^T
+            auto scores = [&](int q, int it) {  // S(it) = Q K(it)^T
                 const int st = it % NS, b = NQ == 2 ? q : it & 1;
                 if (!wait(&k_full[st], (it / NS) & 1)) return;
                 tc_fence_after();
+                const uint64_t q_d = smem_desc_sw128(smem_u32(smem + L.q + (uint32_t)q * C::QBYTES));
                 const uint64_t k_d = smem_desc_sw128(smem_u32(smem + L.k + (uint32_t)st * C::KBYTES));
                 if (one) {
 #pragma unroll
@@ -376,41 +380,47 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                         tc_mma(tmem + C::S_COL + (uint32_t)(b * BN), q_d + ((part * 128u * 128u + k) >> 4),
                                k_d + ((part * (uint32_t)BN * 128u + k) >> 4), id_s, m > 0);
                     }
-                    tc_commit(&k_empty[st]);
                     tc_commit(&s_full[b]);
+                    if (q == NQ - 1) tc_commit(&k_empty[st]);
                 }
                 __syncwarp();
                 issued = true;
             };
-            auto values = [&](int it) {  // O += P(it) V(it)
+            auto values = [&](int q, int it) {  // O += P(it) V(it)
                 const int st = it % NS, b = NQ == 2 ? q : it & 1;
                 const uint32_t n = NQ == 2 ? it : it >> 1;  // how often the buffer was used before
                 if (!wait(&v_full[st], (it / NS) & 1) || !wait(&p_full[b], n & 1)) return;
                 tc_fence_after();
+                const uint32_t o_t = tmem + C::O_COL + (uint32_t)(q * HD);
                 const uint32_t p_t = tmem + C::S_COL + (uint32_t)(b * BN);
                 const uint64_t v_d = v_desc(smem_u32(smem + L.v + (uint32_t)st * C::KBYTES), (uint32_t)BN * 128u);
                 if (one) {
 #pragma unroll
                     for (int m = 0; m < BN / 16; ++m)
                         tc_mma_ts(o_t, p_t + (uint32_t)(m * 8), v_d + ((m * 16u * 128u) >> 4), id_o, it > 0 || m > 0);
-                    tc_commit(&v_empty[st]);
+                    if (q == NQ - 1) tc_commit(&v_empty[st]);
                     if (NQ == 1) tc_commit(&pv_done[0]);
+                    if (it == nt - 1) tc_commit(&o_full[q]);
                 }
                 __syncwarp();
             };
             wait(q_full, 0);
             tc_fence_after();
-            if (ok) scores(0);
+            for (int q = 0; q < NQ; ++q)
+                if (ok) scores(q, 0);
             for (int it = 0; it < nt && ok; ++it) {
-                if (NQ == 1 && it + 1 < nt) scores(it + 1);  // into the other buffer, while softmax works
-                if (ok) values(it);
-                // the scores of the next tile overwrite P: issued after the product that reads it
-                if (NQ == 2 && ok && it + 1 < nt) scores(it + 1);
+                if (NQ == 1 && it + 1 < nt) scores(0, it + 1);  // into the other buffer, while softmax works
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    if (ok) values(q, it);
+                    // the scores of the next tile overwrite P: issued after the product that reads it
+                    if (NQ == 2 && ok && it + 1 < nt) scores(q, it + 1);
+                }
             }
-            if (issued) {
-                if (one) tc_commit(&o_full[q]);
+            if (issued) {  // every MMA retired before TMEM goes
+                if (one) tc_commit(mma_done);
                 __syncwarp();
-                mbar_wait(&o_full[q], 0, nullptr, 0);  // every MMA retired before TMEM goes
+                mbar_wait(mma_done, 0, nullptr, 0);
             }
         }
     } else if (warp < 4 * NQ) {

@@ -10,8 +10,8 @@
 // cores work for one stream, the other's softmax runs.  At head_dim 256 the two outputs would not fit
 // in TMEM beside the scores: one stream of 128 rows with two score buffers.
 //
-// Warps: 0-3 and 4-7 softmax, one thread a row (stream 0, stream 1; at head_dim 256 only 0-3); 8 and 9
-// load K and V; 10 issues the MMAs.
+// Warps: eight softmax warps a stream, two threads a row (half a tile's keys each); then one warp loads K,
+// one V, and one issues the MMAs.
 //   S = Q K^T       A = Q, B = K, both from shared memory (K-major, 128-byte swizzle)
 //   O += P V        A = P from TMEM (16-bit, over the scores it came from), B = V from shared memory
 //                   (N-major: a V row is 64 dims of one key)
@@ -33,12 +33,10 @@
 
 namespace ti {
 
-constexpr int kPreThreads = 384;
-// Registers: the block is launched with 168 a thread (384 x 168 = 64,512); with two streams the
-// loading and issuing warps hand theirs to the softmax warps, which hold a whole row of scores:
-// 128 x 56 + 256 x 224 = 64,512.
-constexpr int kRegsLaunch = 168, kRegsOther = 56, kRegsSoftmax = 224;
-static_assert(128 * kRegsOther + 256 * kRegsSoftmax == kPreThreads * kRegsLaunch, "the shares are what was launched");
+// Registers: with two streams the block is launched with 96 a thread (640 x 96 = 61,440), and the loading and
+// issuing warps hand some of theirs to the softmax warps: 128 x 64 + 512 x 104 = 61,440.
+constexpr int kRegsLaunch = 96, kRegsOther = 64, kRegsSoftmax = 104;
+static_assert(128 * kRegsOther + 512 * kRegsSoftmax == 640 * kRegsLaunch, "the shares are what was launched");
 template <int N>
 TI_DEVICE_INLINE void regs_inc() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -97,7 +95,10 @@ template <int HD>
 struct PreCfg {
     static constexpr int NQ = HD <= 128 ? 2 : 1;    // row tiles (streams) of a CTA
     static constexpr int ROWS = NQ * 128;
+    static constexpr int SW = NQ * 8;               // softmax warps: two threads a row
+    static constexpr int THREADS = SW * 32 + 128;   // + K, V and MMA warps, and an idle one
     static constexpr int BN = HD <= 128 ? 128 : 64;  // keys of a tile
+    static constexpr int COLS = BN / 2;             // keys of a tile that one softmax thread takes
     static constexpr int NB = 2;                    // score buffers: one a stream, or two for the one stream
     static constexpr int NS = HD == 64 ? 4 : 2;     // K stages, and V stages
     static constexpr int PARTS = HD / 64;
@@ -110,7 +111,7 @@ struct PreCfg {
 };
 
 struct PreSmem {
-    uint32_t q, k, v, bar, misc, total;
+    uint32_t q, k, v, bar, misc, xch, total;
 };
 template <int HD>
 __host__ __device__ constexpr PreSmem pre_smem() {
@@ -127,6 +128,8 @@ __host__ __device__ constexpr PreSmem pre_smem() {
     o += 8 * (4 * C::NS + 2 + 8 + 2);
     L.misc = o;  // [0] TMEM base, [1] stop, [2..3] lo, hi
     o += 32;
+    L.xch = o;  // what the two threads of a row tell each other: [2][streams][halves][128]
+    o += 2 * C::NQ * 2 * 128 * 4;
     L.total = o + 1024;
     return L;
 }
@@ -196,12 +199,13 @@ __host__ __device__ constexpr uint32_t pre_idesc(int n, bool b_nmajor) {
 }
 
 template <int HD, class T, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kPreThreads, 1)
+__global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
     k_paged_prefill(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                     const __grid_constant__ PreArgs a) {
     using C = PreCfg<HD>;
     constexpr int BN = C::BN, NS = C::NS, NQ = C::NQ;
     constexpr PreSmem L = pre_smem<HD>();
+    constexpr int kKWarp = C::SW, kVWarp = C::SW + 1, kMmaWarp = C::SW + 2;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L.bar);
@@ -231,9 +235,11 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     const int32_t* table = table_row(a.p.r, s);
     const int n_keys = table ? min(max(kv_len, 0), a.p.r.pt_stride * kPageTokens) : 0;
     int token = 0, head = 0, pos = 0, lo = 0, hi = 0;
-    const bool mine = tid < C::ROWS && tid < n_rows;
+    // (softmax warps 8 q + 4 half + quarter: the row of lane l is 128 q + 32 quarter + l)
+    const int row_id = (warp >> 3) * 128 + (warp & 3) * 32 + lane;
+    const bool mine = warp < C::SW && row_id < n_rows;
     if (mine) {
-        const int r = rt.row0 + tid;
+        const int r = rt.row0 + row_id;
         token = rt.t0 + r / a.group;
         head = hk * a.group + r % a.group;
         pos = kv_len - (rt.t1 - token);
@@ -248,10 +254,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
         mbar_init(v_edge, 1);
         mbar_init(mma_done, 1);
-        mbar_init(q_full, 4 * NQ);  // the softmax warps
+        mbar_init(q_full, C::SW);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);  // the warps of a stream
+            mbar_init(&p_full[i], 8);  // the warps of a stream
             mbar_init(&pv_done[i], 1);
             mbar_init(&o_full[i], 1);
         }
@@ -260,7 +266,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         range[1] = 0;
         fence_barrier_init();
     }
-    if (warp == 10) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)misc)),
                      "r"(512u)
                      : "memory");
@@ -298,8 +304,8 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
         __syncwarp();
     };
-    if (NQ == 2 && warp >= 8) regs_dec<kRegsOther>();
-    if (warp == 8) {
+    if (NQ == 2 && warp >= C::SW) regs_dec<kRegsOther>();
+    if (warp == kKWarp) {
         // ---------------------------------------------------------- K
         for (int it = 0; it < nt; ++it) {
             const int st = it % NS;
@@ -314,7 +320,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
         if (misc[1])  // a wait gave up: copies in flight land before the block ends
             for (int i = 0; i < NS; ++i) mbar_wait_for(&k_full[i], 0, nullptr, 0, 1000000);
-    } else if (warp == 9) {
+    } else if (warp == kVWarp) {
         // ---------------------------------------------------------- V
         int edges = 0;
         for (int it = 0; it < nt; ++it) {
@@ -350,13 +356,13 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
         if (misc[1])
             for (int i = 0; i < NS; ++i) mbar_wait_for(&v_full[i], 0, nullptr, 0, 1000000);
-    } else if (warp >= 10) {
+    } else if (warp == kMmaWarp) {
         // ---------------------------------------------------------- MMA issue
         // One warp for both streams: a stream's P V and next scores are issued together, so the
         // tensor cores finish one stream's batch while the other's softmax runs.  With a warp a stream
         // the batches interleave, both streams wait for both, and then both softmaxes
         // compete for the exponentials (4,800 against 3,500 cycles a pair of tiles).
-        if (warp == 10 && nt > 0) {
+        if (nt > 0) {
             const uint32_t id_s = pre_idesc<T>(BN, false), id_o = pre_idesc<T>(HD, true);
             const bool one = elect_one();
             bool ok = true, issued = false;
@@ -423,19 +429,26 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                 mbar_wait(mma_done, 0, nullptr, 0);
             }
         }
-    } else if (warp < 4 * NQ) {
-        // ---------------------------------------------------------- softmax: one thread a row
+    } else if (warp < C::SW) {
+        // ---------------------------------------------------------- softmax: two threads a row, half a tile's keys each
+        // (one thread a row leaves one warp a scheduler at work while the other stream waits: its
+        // latencies show, 536 against OTHERus for 8,192 causal tokens)
         if (NQ == 2) regs_inc<kRegsSoftmax>();
-        const int q = warp >> 2;
+        constexpr int N = C::COLS;
+        const int q = warp >> 3, half = (warp >> 2) & 1, col = half * N;
+        float* xch = reinterpret_cast<float*>(smem + L.xch);
+        // (buffer, half) of this row; the two warps of 32 rows meet at a barrier of their own
+        auto xrow = [&](int buf, int h) { return xch + ((buf * NQ + q) * 2 + h) * 128 + (warp & 3) * 32 + lane; };
+        auto pair_bar = [&] { named_bar(1 + q * 4 + (warp & 3), 64); };
         const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         // ---- Q rows into shared memory (rows past the end are zero)
         {
             const T* src = reinterpret_cast<const T*>(a.p.q) + (mine ? (int64_t)token * a.p.q_stride + (int64_t)head * HD : 0);
             uint8_t* qt = smem + L.q + (uint32_t)q * C::QBYTES;
             constexpr int CH = HD / 8;        // 16-byte chunks of a row
-            constexpr int RP = 32 / (CH < 32 ? CH : 32);  // rows at a time
+            constexpr int RP = 32 / CH;       // rows at a time
             const int rl = lane / CH, c = lane % CH;
-            for (int i = 0; i < 32; i += RP) {
+            for (int i = half * 16; i < half * 16 + 16; i += RP) {
                 const T* p = reinterpret_cast<const T*>(
                     __shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, i + rl));
                 const bool have = __shfl_sync(0xffffffffu, (int)mine, i + rl);
@@ -473,26 +486,23 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         for (int it = 0; it < nt; ++it) {
             const int b = NQ == 2 ? q : it & 1;
             const uint32_t n = NQ == 2 ? it : it >> 1;
-            const int k0 = (j0 + it) * BN;
-            if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&s_full[b], n & 1, nullptr, 0))) {
-                misc[1] = 1;
-                break;
-            }
+            const int k0 = (j0 + it) * BN + col;  // this thread's first key
+            if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&s_full[b], n & 1, nullptr, 0))) misc[1] = 1;
             tc_fence_after();
-            float x[BN];
+            float x[N];
 #pragma unroll
-            for (int c = 0; c < BN; c += 32) tmem_ld32_async(t_lane + C::S_COL + (uint32_t)(b * BN + c), x + c);
-            tmem_ld_done<BN>(x);
+            for (int c = 0; c < N; c += 32) tmem_ld32_async(t_lane + C::S_COL + (uint32_t)(b * BN + col + c), x + c);
+            tmem_ld_done<N>(x);
             // a tile that some row of the warp sees in part
-            const bool edge = !__all_sync(0xffffffffu, lo <= k0 && hi >= k0 + BN);
+            const bool edge = !__all_sync(0xffffffffu, lo <= k0 && hi >= k0 + N);
             auto row_max = [&] {
                 float m4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int c = 4; c < BN - 4; c += 8)
+                for (int c = 4; c < N - 4; c += 8)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) m4[k] = max3(m4[k], x[c + k], x[c + 4 + k]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], x[BN - 4 + k]);
+                for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], x[N - 4 + k]);
                 return fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
             };
             auto poly = [&](float2 v, float2 add) {  // z of a pair + add
@@ -509,11 +519,11 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                 mx = row_max();
                 float n4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int c = 4; c < BN - 4; c += 8)
+                for (int c = 4; c < N - 4; c += 8)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) n4[k] = min3(n4[k], x[c + k], x[c + 4 + k]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) n4[k] = fminf(n4[k], x[BN - 4 + k]);
+                for (int k = 0; k < 4; ++k) n4[k] = fminf(n4[k], x[N - 4 + k]);
                 const float mn = fminf(min3(n4[0], n4[1], n4[2]), n4[3]);
                 // (max and min drop a NaN, and both ways give NaN for it)
                 small = !edge && __all_sync(0xffffffffu, mx <= s_max && mn >= -s_max);
@@ -521,7 +531,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                     mx = poly(make_float2(mx, 0.f), dup2(0.f)).x;  // monotonic: the maximum of the capped scores
                 } else if (small) {
 #pragma unroll
-                    for (int c = 0; c < BN; c += 2) {
+                    for (int c = 0; c < N; c += 2) {
                         const float2 y = poly(make_float2(x[c], x[c + 1]), dup2(0.f));
                         x[c] = y.x;
                         x[c + 1] = y.y;
@@ -530,46 +540,47 @@ __global__ void __launch_bounds__(kPreThreads, 1)
                     // cap tanh(u) = cap - 2 cap / (e^(2u) + 1), whatever u is
                     const float c_in = 2.f * kLog2E * u1;
 #pragma unroll
-                    for (int c = 0; c < BN; ++c) x[c] = fmaf(-2.f * cap2, rcp_approx(ex2(x[c] * c_in) + 1.f), cap2);
+                    for (int c = 0; c < N; ++c) x[c] = fmaf(-2.f * cap2, rcp_approx(ex2(x[c] * c_in) + 1.f), cap2);
                 }
             }
             if constexpr (BIAS) {
                 const float d0 = (float)(pos - k0);
-                if (!edge && __all_sync(0xffffffffu, pos >= k0 + BN - 1 || !mine)) {
+                if (!edge && __all_sync(0xffffffffu, pos >= k0 + N - 1 || !mine)) {
                     // every key is at or before the row: -slope (i - j) is a line in j
                     const float2 sl = dup2(slope2), sc = dup2(CAP ? 1.f : scale2);
                     const float b0 = -slope2 * d0;
 #pragma unroll
-                    for (int c = 0; c < BN; c += 2) {
+                    for (int c = 0; c < N; c += 2) {
                         const float2 y = fma2(make_float2(x[c], x[c + 1]), sc, fma2(sl, make_float2((float)c, (float)(c + 1)), dup2(b0)));
                         x[c] = y.x;
                         x[c + 1] = y.y;
                     }
                 } else {
 #pragma unroll
-                    for (int c = 0; c < BN; ++c) x[c] = fmaf(-slope2, fabsf(d0 - (float)c), CAP ? x[c] : x[c] * scale2);
+                    for (int c = 0; c < N; ++c) x[c] = fmaf(-slope2, fabsf(d0 - (float)c), CAP ? x[c] : x[c] * scale2);
                 }
             }
             if (edge) {
                 const int cl = lo - k0, ch = hi - k0;
 #pragma unroll
-                for (int c = 0; c < BN; ++c) x[c] = c >= cl && c < ch ? x[c] : -INFINITY;
+                for (int c = 0; c < N; ++c) x[c] = c >= cl && c < ch ? x[c] : -INFINITY;
             }
             if (!CAP || BIAS || !small) mx = row_max() * mult;
+            // the other half's maximum; past the barrier both threads have read their scores, which P overwrites
+            *xrow(it & 1, half) = mx;
+            pair_bar();
+            mx = fmaxf(mx, *xrow(it & 1, half ^ 1));
             // ---- lazily rescaled maximum
             bool grow = mx > m + 8.f;  // (m = -inf: the first keys of the row)
             if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
                 if (NQ == 1 && it > 0) {  // with two streams s_full(it) already says that P V (it - 1) is done
-                    if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&pv_done[0], (it - 1) & 1, nullptr, 0))) {
-                        misc[1] = 1;
-                        break;
-                    }
+                    if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&pv_done[0], (it - 1) & 1, nullptr, 0))) misc[1] = 1;
                     tc_fence_after();
                 }
                 const float f = grow ? ex2(m - mx) : 1.f;
                 l *= f;
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
+                for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                     float o[32];
                     const uint32_t at = t_lane + C::O_COL + (uint32_t)(q * HD + c);
                     uint32_t w[32];
@@ -584,18 +595,17 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             float2 sum = dup2(0.f);
             const float2 mu = dup2(-u), mm = dup2(mult);
             auto exps = [&](auto&& arg) {
+                uint32_t w[N / 2];
 #pragma unroll
-                for (int h = 0; h < BN; h += 64) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        const float2 y = arg(make_float2(x[h + 2 * c], x[h + 2 * c + 1]));
-                        const float2 p = make_float2(ex2(y.x), ex2(y.y));
-                        sum = add2(sum, p);
-                        w[c] = Elem<T>::pack(p.x, p.y);
-                    }
-                    tmem_st32(t_lane + C::S_COL + (uint32_t)(b * BN + h / 2), w);
+                for (int c = 0; c < N / 2; ++c) {
+                    const float2 y = arg(make_float2(x[2 * c], x[2 * c + 1]));
+                    const float2 p = make_float2(ex2(y.x), ex2(y.y));
+                    sum = add2(sum, p);
+                    w[c] = Elem<T>::pack(p.x, p.y);
                 }
+                const uint32_t at = t_lane + C::S_COL + (uint32_t)(b * BN + col / 2);
+                if constexpr (N == 64) tmem_st32(at, w);
+                else tmem_st16(at, w);
             };
             if (CAP && !BIAS && small) exps([&](float2 v) { return poly(v, mu); });
             else exps([&](float2 v) { return fma2(v, mm, mu); });
@@ -605,7 +615,10 @@ __global__ void __launch_bounds__(kPreThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[b]);
         }
-        // ---- output rows
+        // ---- output rows: each thread half of the dims; the sum of both halves
+        *xrow(nt & 1, half) = l;
+        pair_bar();
+        l += *xrow(nt & 1, half ^ 1);
         bool good = true;
         if (nt > 0) {
             good = !__any_sync(0xffffffffu, misc[1] || !mbar_wait(&o_full[q], 0, nullptr, 0));
@@ -613,9 +626,9 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         }
         if (a.splits > 1) {
             const int64_t row = ((int64_t)blockIdx.z * a.p.r.n_tokens + token) * a.p.n_heads + head;
-            if (mine) reinterpret_cast<float2*>(a.part_ml)[row] = nt > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+            if (mine && half == 0) reinterpret_cast<float2*>(a.part_ml)[row] = nt > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
             if (nt > 0 && good) {
-                for (int c = 0; c < HD; c += 32) {
+                for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                     float o[32];
                     tmem_ld32(t_lane + C::O_COL + (uint32_t)(q * HD + c), o);
                     if (mine)
@@ -628,7 +641,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
         } else {
             T* dst = reinterpret_cast<T*>(a.p.out) + (int64_t)token * a.p.out_stride + (int64_t)head * HD;
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            for (int c = 0; c < HD; c += 32) {
+            for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                 float o[32];
                 if (nt > 0) tmem_ld32(t_lane + C::O_COL + (uint32_t)(q * HD + c), o);
                 uint32_t w[16];
@@ -655,7 +668,7 @@ __global__ void __launch_bounds__(kPreThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 10) {
+    if (warp == kMmaWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
@@ -739,7 +752,7 @@ cudaError_t paged_prefill_launch(const PagedAttn& p, int dev, cudaStream_t s) {
         a.part_ml = scratch + n * p.hd;
     }
     void* args[] = {&tk, &tv, &a};
-    e = launch_pdl(f, dim3((unsigned)tiles, p.n_kv, a.splits), dim3(kPreThreads), smem, s, args, false);
+    e = launch_pdl(f, dim3((unsigned)tiles, p.n_kv, a.splits), dim3(p.hd <= 128 ? PreCfg<128>::THREADS : PreCfg<256>::THREADS), smem, s, args, false);
     if (a.splits > 1) {
         if (e == cudaSuccess) {
             void* jargs[] = {&a};

@@ -223,9 +223,11 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
     int* range = reinterpret_cast<int*>(smem + L.misc) + 2;
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform, and known to be
-    const int hk = blockIdx.y;
+    // kv heads innermost: the longest row tiles of every head start first (head after head, the last
+    // head's long tiles started late and ran alone)
+    const int hk = blockIdx.x % a.p.n_kv;
 
-    const RowTile rt = find_rows<C::ROWS>(a, blockIdx.x);
+    const RowTile rt = find_rows<C::ROWS>(a, blockIdx.x / a.p.n_kv);
     if (rt.seq < 0) return;  // the whole block
     const int s = rt.seq;
     const int n_rows = (rt.t1 - rt.t0) * a.group - rt.row0;  // rows of the sequence from the tile's first on
@@ -730,7 +732,7 @@ cudaError_t paged_prefill_launch(const PagedAttn& p, int dev, cudaStream_t s) {
     const int rows = p.hd <= 128 ? 256 : 128, bn = p.hd <= 128 ? 128 : 64;
     // every sequence may end in a part of a tile; CTAs past the last tile return at once
     const int64_t tiles = (int64_t)p.r.n_tokens * a.group / rows + std::min(p.r.n_seqs, p.r.n_tokens);
-    if (tiles > INT32_MAX) return cudaErrorInvalidValue;
+    if (tiles * p.n_kv > INT32_MAX) return cudaErrorInvalidValue;
     // key tiles are divided when the row tiles alone leave SMs idle, down to four tiles a CTA
     const int64_t span = p.f.window > 0 ? std::min<int64_t>(p.max_len, (int64_t)p.f.window + rows) : p.max_len;
     const int64_t ctas = tiles * p.n_kv, key_tiles = (span + bn - 1) / bn;
@@ -752,7 +754,7 @@ cudaError_t paged_prefill_launch(const PagedAttn& p, int dev, cudaStream_t s) {
         a.part_ml = scratch + n * p.hd;
     }
     void* args[] = {&tk, &tv, &a};
-    e = launch_pdl(f, dim3((unsigned)tiles, p.n_kv, a.splits), dim3(p.hd <= 128 ? PreCfg<128>::THREADS : PreCfg<256>::THREADS), smem, s, args, false);
+    e = launch_pdl(f, dim3((unsigned)(tiles * p.n_kv), 1, a.splits), dim3(p.hd <= 128 ? PreCfg<128>::THREADS : PreCfg<256>::THREADS), smem, s, args, false);
     if (a.splits > 1) {
         if (e == cudaSuccess) {
             void* jargs[] = {&a};

@@ -11,6 +11,16 @@ namespace ti {
 constexpr int kPageTokens = 16;
 constexpr float kLog2E = 1.4426950408889634f;
 
+// Bounded wait of a pipeline role: false once `stop` is set by a wait that gave up (its own or another
+// role's).  The flag is read only after a poll has failed: while MMAs stream operands out of shared
+// memory every other access to it takes some 200 cycles.
+TI_DEVICE_INLINE bool pipe_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*stop == 0 && mbar_wait(bar, parity, nullptr, 0)) return true;
+    *stop = 1;
+    return false;
+}
+
 // ------------------------------------------------------------------ 16-bit element types
 template <class T>
 struct Elem;

@@ -263,10 +263,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                     ahead = p + 32 + lane < p1 ? ids[p + 32 + lane] : 0;
                 }
                 const int id = __shfl_sync(0xffffffffu, cur, (i + lane) & 31);  // lane l: page p + l
-                if (__any_sync(0xffffffffu, *stop || !mbar_wait(&empty[slot], ((it / NS) & 1) ^ 1, nullptr, 0))) {
-                    *stop = 1;
-                    continue;
-                }
+                if (!__all_sync(0xffffffffu, pipe_wait(&empty[slot], ((it / NS) & 1) ^ 1, stop))) continue;
                 if (lane == 0) mbar_arrive_expect_tx(&full[slot], (uint32_t)n * HD * 32u);
                 __syncwarp();
                 if (lane < n) {
@@ -349,8 +346,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
             const int tok0 = (x.pg0 + p0 + st * CP) * kPageTokens;  // key of stage row 0
             const int rows = min(CP, p1 - p0 - st * CP) * kPageTokens;
             const int jlo = max(x.lo - tok0, 0), jhi = min(x.hi - tok0, rows);
-            const bool bad = __any_sync(0xffffffffu, *stop || !mbar_wait(&full[slot], (gi / NS) & 1, nullptr, 0));
-            if (bad) *stop = 1;
+            const bool bad = !__all_sync(0xffffffffu, pipe_wait(&full[slot], (gi / NS) & 1, stop));
             if (j0 + 16 > jlo && j0 < jhi && !bad) {  // warp-uniform
                 const bool edge = j0 < jlo || j0 + 16 > jhi;
                 if (edge) {

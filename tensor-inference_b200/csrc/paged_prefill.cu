@@ -70,9 +70,15 @@ TI_DEVICE_INLINE float2 add2(float2 a, float2 b) {
     return d;
 }
 TI_DEVICE_INLINE float2 dup2(float v) { return make_float2(v, v); }
+// (a NaN stays one)
 TI_DEVICE_INLINE float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+TI_DEVICE_INLINE float max2(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
 TI_DEVICE_INLINE float min3(float a, float b, float c) {
@@ -124,8 +130,9 @@ __host__ __device__ constexpr PreSmem pre_smem() {
     o += C::NS * C::KBYTES;
     L.v = o;
     o += C::NS * C::KBYTES;
-    L.bar = o;  // k_full, k_empty, v_full, v_empty [NS]; v_edge, q_full; s_full, p_full, pv_done, o_full [2]; mma_done
-    o += 8 * (4 * C::NS + 2 + 8 + 2);
+    L.bar = o;  // k_full, k_empty, v_full, v_empty [NS]; v_edge, q_full; s_full, p_full, p_half, pv_done, o_full [2];
+                  // mma_done
+    o += 8 * (4 * C::NS + 2 + 10 + 2);
     L.misc = o;  // [0] TMEM base, [1] stop, [2..3] lo, hi
     o += 32;
     L.xch = o;  // what the two threads of a row tell each other: [2][streams][halves][128]
@@ -216,10 +223,12 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
     uint64_t* q_full = v_edge + 1;
     uint64_t* s_full = q_full + 1;
     uint64_t* p_full = s_full + 2;
-    uint64_t* pv_done = p_full + 2;
+    uint64_t* p_half = p_full + 2;
+    uint64_t* pv_done = p_half + 2;
     uint64_t* o_full = pv_done + 2;
     uint64_t* mma_done = o_full + 2;
     volatile int* misc = reinterpret_cast<volatile int*>(smem + L.misc);
+    volatile int* stop = misc + 1;
     int* range = reinterpret_cast<int*>(smem + L.misc) + 2;
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform, and known to be
@@ -260,10 +269,11 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 8);  // the warps of a stream
+            mbar_init(&p_half[i], 8);
             mbar_init(&pv_done[i], 1);
             mbar_init(&o_full[i], 1);
         }
-        misc[1] = 0;
+        *stop = 0;
         range[0] = INT32_MAX;
         range[1] = 0;
         fence_barrier_init();
@@ -314,13 +324,10 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             const int page = (j0 + it) * C::PAGES + lane;
             const int id = lane < C::PAGES && page * kPageTokens < n_keys ? table[page] : -1;
             const int row = id >= 0 && id < a.p.r.n_pages ? (id * a.p.n_kv + hk) * kPageTokens : a.cache_rows;
-            if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&k_empty[st], ((it / NS) & 1) ^ 1, nullptr, 0))) {
-                misc[1] = 1;
-                break;
-            }
+            if (!__all_sync(0xffffffffu, pipe_wait(&k_empty[st], ((it / NS) & 1) ^ 1, stop))) break;
             load_tile(smem + L.k + (uint32_t)st * C::KBYTES, &tk, row, &k_full[st]);
         }
-        if (misc[1])  // a wait gave up: copies in flight land before the block ends
+        if (*stop)  // a wait gave up: copies in flight land before the block ends
             for (int i = 0; i < NS; ++i) mbar_wait_for(&k_full[i], 0, nullptr, 0, 1000000);
     } else if (warp == kVWarp) {
         // ---------------------------------------------------------- V
@@ -330,10 +337,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             const int page = (j0 + it) * C::PAGES + lane;
             const int id = lane < C::PAGES && page * kPageTokens < n_keys ? table[page] : -1;
             const int row = id >= 0 && id < a.p.r.n_pages ? (id * a.p.n_kv + hk) * kPageTokens : a.cache_rows;
-            if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&v_empty[st], ((it / NS) & 1) ^ 1, nullptr, 0))) {
-                misc[1] = 1;
-                break;
-            }
+            if (!__all_sync(0xffffffffu, pipe_wait(&v_empty[st], ((it / NS) & 1) ^ 1, stop))) break;
             // a tile with keys that no row sees: those rows of V must be finite (their
             // probabilities are zero), so they are zeroed before the MMAs may read the tile
             const bool edge = k0 < key_lo || k0 + BN > key_hi;
@@ -341,10 +345,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             uint8_t* vt = smem + L.v + (uint32_t)st * C::KBYTES;
             load_tile(vt, &tv, row, bar);
             if (edge) {
-                if (__any_sync(0xffffffffu, !mbar_wait(v_edge, edges & 1, nullptr, 0))) {
-                    misc[1] = 1;
-                    break;
-                }
+                if (!__all_sync(0xffffffffu, pipe_wait(v_edge, edges & 1, stop))) break;
                 ++edges;
                 for (int c = lane; c < BN * C::PARTS * 8; c += 32) {
                     const int r = (c >> 3) % BN;
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 if (lane == 0) mbar_arrive(&v_full[st]);
             }
         }
-        if (misc[1])
+        if (*stop)
             for (int i = 0; i < NS; ++i) mbar_wait_for(&v_full[i], 0, nullptr, 0, 1000000);
     } else if (warp == kMmaWarp) {
         // ---------------------------------------------------------- MMA issue
@@ -369,15 +370,13 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             const bool one = elect_one();
             bool ok = true, issued = false;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
-                if (ok && !__all_sync(0xffffffffu, !misc[1] && mbar_wait(bar, parity, nullptr, 0))) {
-                    misc[1] = 1;
-                    ok = false;
-                }
+                ok = ok && __all_sync(0xffffffffu, pipe_wait(bar, parity, stop));
                 return ok;
             };
             auto scores = [&](int q, int it) {  // S(it) = Q K(it)^T
                 const int st = it % NS, b = NQ == 2 ? q : it & 1;
-                if (!wait(&k_full[st], (it / NS) & 1)) return;
+                // (the other stream's turn found the tile there already)
+                if (q == 0 && !wait(&k_full[st], (it / NS) & 1)) return;
                 tc_fence_after();
                 const uint64_t q_d = smem_desc_sw128(smem_u32(smem + L.q + (uint32_t)q * C::QBYTES));
                 const uint64_t k_d = smem_desc_sw128(smem_u32(smem + L.k + (uint32_t)st * C::KBYTES));
@@ -397,15 +396,26 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             auto values = [&](int q, int it) {  // O += P(it) V(it)
                 const int st = it % NS, b = NQ == 2 ? q : it & 1;
                 const uint32_t n = NQ == 2 ? it : it >> 1;  // how often the buffer was used before
-                if (!wait(&v_full[st], (it / NS) & 1) || !wait(&p_full[b], n & 1)) return;
+                if (q == 0 && !wait(&v_full[st], (it / NS) & 1)) return;
+                if (!wait(&p_half[b], n & 1)) return;
                 tc_fence_after();
                 const uint32_t o_t = tmem + C::O_COL + (uint32_t)(q * HD);
                 const uint32_t p_t = tmem + C::S_COL + (uint32_t)(b * BN);
                 const uint64_t v_d = v_desc(smem_u32(smem + L.v + (uint32_t)st * C::KBYTES), (uint32_t)BN * 128u);
-                if (one) {
+                // the first half of each softmax thread's keys, then the second
+                constexpr int KS = BN / 16;
+                auto steps = [&](int piece) {
 #pragma unroll
-                    for (int m = 0; m < BN / 16; ++m)
-                        tc_mma_ts(o_t, p_t + (uint32_t)(m * 8), v_d + ((m * 16u * 128u) >> 4), id_o, it > 0 || m > 0);
+                    for (int m = 0; m < KS; ++m)
+                        if ((m % (KS / 2) >= KS / 4) == (piece == 1))
+                            tc_mma_ts(o_t, p_t + (uint32_t)(m * 8), v_d + ((m * 16u * 128u) >> 4), id_o, it > 0 || m > 0);
+                };
+                if (one) steps(0);
+                __syncwarp();
+                if (!wait(&p_full[b], n & 1)) return;
+                tc_fence_after();
+                if (one) {
+                    steps(1);
                     if (q == NQ - 1) tc_commit(&v_empty[st]);
                     if (NQ == 1) tc_commit(&pv_done[0]);
                     if (it == nt - 1) tc_commit(&o_full[q]);
@@ -489,7 +499,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             const int b = NQ == 2 ? q : it & 1;
             const uint32_t n = NQ == 2 ? it : it >> 1;
             const int k0 = (j0 + it) * BN + col;  // this thread's first key
-            if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&s_full[b], n & 1, nullptr, 0))) misc[1] = 1;
+            pipe_wait(&s_full[b], n & 1, stop);
+            __syncwarp();
             tc_fence_after();
             float x[N];
 #pragma unroll
@@ -504,8 +515,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) m4[k] = max3(m4[k], x[c + k], x[c + 4 + k]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], x[N - 4 + k]);
-                return fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
+                for (int k = 0; k < 4; ++k) m4[k] = max2(m4[k], x[N - 4 + k]);
+                return max2(max3(m4[0], m4[1], m4[2]), m4[3]);
             };
             auto poly = [&](float2 v, float2 add) {  // z of a pair + add
                 const float2 z = mul2(v, v);
@@ -527,7 +538,6 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) n4[k] = fminf(n4[k], x[N - 4 + k]);
                 const float mn = fminf(min3(n4[0], n4[1], n4[2]), n4[3]);
-                // (max and min drop a NaN, and both ways give NaN for it)
                 small = !edge && __all_sync(0xffffffffu, mx <= s_max && mn >= -s_max);
                 if (small && !BIAS) {
                     mx = poly(make_float2(mx, 0.f), dup2(0.f)).x;  // monotonic: the maximum of the capped scores
@@ -571,12 +581,13 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             // the other half's maximum; past the barrier both threads have read their scores, which P overwrites
             *xrow(it & 1, half) = mx;
             pair_bar();
-            mx = fmaxf(mx, *xrow(it & 1, half ^ 1));
+            mx = max2(mx, *xrow(it & 1, half ^ 1));
             // ---- lazily rescaled maximum
             bool grow = mx > m + 8.f;  // (m = -inf: the first keys of the row)
             if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
                 if (NQ == 1 && it > 0) {  // with two streams s_full(it) already says that P V (it - 1) is done
-                    if (__any_sync(0xffffffffu, misc[1] || !mbar_wait(&pv_done[0], (it - 1) & 1, nullptr, 0))) misc[1] = 1;
+                    pipe_wait(&pv_done[0], (it - 1) & 1, stop);
+                    __syncwarp();
                     tc_fence_after();
                 }
                 const float f = grow ? ex2(m - mx) : 1.f;
@@ -596,26 +607,33 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             const float u = m == -INFINITY ? 0.f : m;
             float2 sum = dup2(0.f);
             const float2 mu = dup2(-u), mm = dup2(mult);
+            auto ready = [&](uint64_t* bar) {  // the P stored so far may be read
+                tmem_st_done();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar);
+            };
             auto exps = [&](auto&& arg) {
-                uint32_t w[N / 2];
 #pragma unroll
-                for (int c = 0; c < N / 2; ++c) {
-                    const float2 y = arg(make_float2(x[2 * c], x[2 * c + 1]));
-                    const float2 p = make_float2(ex2(y.x), ex2(y.y));
-                    sum = add2(sum, p);
-                    w[c] = Elem<T>::pack(p.x, p.y);
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[N / 4];
+#pragma unroll
+                    for (int c = 0; c < N / 4; ++c) {
+                        const int k = h * (N / 2) + 2 * c;
+                        const float2 y = arg(make_float2(x[k], x[k + 1]));
+                        const float2 p = make_float2(ex2(y.x), ex2(y.y));
+                        sum = add2(sum, p);
+                        w[c] = Elem<T>::pack(p.x, p.y);
+                    }
+                    const uint32_t at = t_lane + C::S_COL + (uint32_t)(b * BN + col / 2 + h * (N / 4));
+                    if constexpr (N == 64) tmem_st16(at, w);
+                    else tmem_st8(at, w);
+                    ready(h == 0 ? &p_half[b] : &p_full[b]);
                 }
-                const uint32_t at = t_lane + C::S_COL + (uint32_t)(b * BN + col / 2);
-                if constexpr (N == 64) tmem_st32(at, w);
-                else tmem_st16(at, w);
             };
             if (CAP && !BIAS && small) exps([&](float2 v) { return poly(v, mu); });
             else exps([&](float2 v) { return fma2(v, mm, mu); });
             l += sum.x + sum.y;
-            tmem_st_done();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[b]);
         }
         // ---- output rows: each thread half of the dims; the sum of both halves
         *xrow(nt & 1, half) = l;
@@ -623,7 +641,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         l += *xrow(nt & 1, half ^ 1);
         bool good = true;
         if (nt > 0) {
-            good = !__any_sync(0xffffffffu, misc[1] || !mbar_wait(&o_full[q], 0, nullptr, 0));
+            good = __all_sync(0xffffffffu, pipe_wait(&o_full[q], 0, stop));
             tc_fence_after();
         }
         if (a.splits > 1) {

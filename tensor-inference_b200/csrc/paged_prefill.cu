@@ -70,22 +70,9 @@ TI_DEVICE_INLINE float2 add2(float2 a, float2 b) {
     return d;
 }
 TI_DEVICE_INLINE float2 dup2(float v) { return make_float2(v, v); }
-// (a NaN stays one)
-TI_DEVICE_INLINE float max3(float a, float b, float c) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-TI_DEVICE_INLINE float max2(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-TI_DEVICE_INLINE float min3(float a, float b, float c) {
-    float d;
-    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
+// of three in one instruction
+TI_DEVICE_INLINE float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+TI_DEVICE_INLINE float min3(float a, float b, float c) { return fminf(fminf(a, b), c); }
 TI_DEVICE_INLINE float rcp_approx(float v) {
     float d;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(v));
@@ -111,7 +98,8 @@ struct PreCfg {
     static constexpr int PAGES = BN / kPageTokens;
     static constexpr uint32_t QBYTES = 128u * HD * 2;  // one row tile of Q
     static constexpr uint32_t KBYTES = (uint32_t)BN * HD * 2;
-    static constexpr uint32_t S_COL = 0;            // score buffer b at b * BN, P over its first half
+    static constexpr uint32_t S_COL = 0;            // score buffer b at b * BN; P over the scores, each softmax
+                                                    // thread's over the first half of its own
     static constexpr uint32_t O_COL = 256;          // output of stream s at O_COL + s * HD
     static_assert(NB * BN <= (int)O_COL && (int)O_COL + NQ * HD <= 512, "TMEM columns");
 };
@@ -408,7 +396,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
 #pragma unroll
                     for (int m = 0; m < KS; ++m)
                         if ((m % (KS / 2) >= KS / 4) == (piece == 1))
-                            tc_mma_ts(o_t, p_t + (uint32_t)(m * 8), v_d + ((m * 16u * 128u) >> 4), id_o, it > 0 || m > 0);
+                            tc_mma_ts(o_t, p_t + (uint32_t)(m / (KS / 2) * (BN / 2) + m % (KS / 2) * 8), v_d + ((m * 16u * 128u) >> 4), id_o, it > 0 || m > 0);
                 };
                 if (one) steps(0);
                 __syncwarp();
@@ -494,7 +482,10 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             lo = 0;
             hi = INT32_MAX;
         }
-        float m = -INFINITY, l = 0.f;
+        // Capped scores lie within the cap, and bf16 has fp32's range: as long as 2^(+-cap2), summed over
+        // any length, stays well inside it, no maximum is needed (m = 0)
+        const bool flat = CAP && !BIAS && Elem<T>::kUmmaFmt == 1 && cap2 <= 80.f;
+        float m = flat ? 0.f : -INFINITY, l = 0.f;
         for (int it = 0; it < nt; ++it) {
             const int b = NQ == 2 ? q : it & 1;
             const uint32_t n = NQ == 2 ? it : it >> 1;
@@ -508,16 +499,19 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             tmem_ld_done<N>(x);
             // a tile that some row of the warp sees in part
             const bool edge = !__all_sync(0xffffffffu, lo <= k0 && hi >= k0 + N);
-            auto row_max = [&] {
-                float m4[4] = {x[0], x[1], x[2], x[3]};
+            // of this thread's scores: op is max3 / min3, f what is taken of each
+            auto reduce = [&](auto&& op, auto&& f) {
+                float r[4] = {f(x[0]), f(x[1]), f(x[2]), f(x[3])};
 #pragma unroll
                 for (int c = 4; c < N - 4; c += 8)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) m4[k] = max3(m4[k], x[c + k], x[c + 4 + k]);
+                    for (int k = 0; k < 4; ++k) r[k] = op(r[k], f(x[c + k]), f(x[c + 4 + k]));
 #pragma unroll
-                for (int k = 0; k < 4; ++k) m4[k] = max2(m4[k], x[N - 4 + k]);
-                return max2(max3(m4[0], m4[1], m4[2]), m4[3]);
+                for (int k = 0; k < 4; ++k) r[k] = op(r[k], r[k], f(x[N - 4 + k]));
+                return op(op(r[0], r[1], r[2]), r[3], r[3]);
             };
+            auto same = [](float v) { return v; };
+            auto row_max = [&] { return reduce(max3, same); };
             auto poly = [&](float2 v, float2 add) {  // z of a pair + add
                 const float2 z = mul2(v, v);
                 float2 h = fma2(dup2(c4), z, dup2(c3));
@@ -527,20 +521,16 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 return fma2(h, v, add);
             };
             bool small = false;  // capped scores within the polynomial's range
-            float mx;
+            float mx = 0.f;
             if constexpr (CAP) {
-                mx = row_max();
-                float n4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int c = 4; c < N - 4; c += 8)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) n4[k] = min3(n4[k], x[c + k], x[c + 4 + k]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) n4[k] = fminf(n4[k], x[N - 4 + k]);
-                const float mn = fminf(min3(n4[0], n4[1], n4[2]), n4[3]);
-                small = !edge && __all_sync(0xffffffffu, mx <= s_max && mn >= -s_max);
+                if (flat) {
+                    small = !edge && __all_sync(0xffffffffu, reduce(max3, [](float v) { return fabsf(v); }) <= s_max);
+                } else {
+                    mx = row_max();
+                    small = !edge && __all_sync(0xffffffffu, mx <= s_max && reduce(min3, same) >= -s_max);
+                }
                 if (small && !BIAS) {
-                    mx = poly(make_float2(mx, 0.f), dup2(0.f)).x;  // monotonic: the maximum of the capped scores
+                    if (!flat) mx = poly(make_float2(mx, 0.f), dup2(0.f)).x;  // monotonic: the maximum of the capped scores
                 } else if (small) {
 #pragma unroll
                     for (int c = 0; c < N; c += 2) {
@@ -577,33 +567,34 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
 #pragma unroll
                 for (int c = 0; c < N; ++c) x[c] = c >= cl && c < ch ? x[c] : -INFINITY;
             }
-            if (!CAP || BIAS || !small) mx = row_max() * mult;
-            // the other half's maximum; past the barrier both threads have read their scores, which P overwrites
-            *xrow(it & 1, half) = mx;
-            pair_bar();
-            mx = max2(mx, *xrow(it & 1, half ^ 1));
-            // ---- lazily rescaled maximum
-            bool grow = mx > m + 8.f;  // (m = -inf: the first keys of the row)
-            if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
-                if (NQ == 1 && it > 0) {  // with two streams s_full(it) already says that P V (it - 1) is done
-                    pipe_wait(&pv_done[0], (it - 1) & 1, stop);
-                    __syncwarp();
-                    tc_fence_after();
+            if (!flat) {
+                if (!CAP || BIAS || !small) mx = row_max() * mult;
+                *xrow(it & 1, half) = mx;  // the other half's maximum
+                pair_bar();
+                mx = fmaxf(mx, *xrow(it & 1, half ^ 1));
+                // ---- lazily rescaled maximum
+                bool grow = mx > m + 8.f;  // (m = -inf: the first keys of the row)
+                if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
+                    if (NQ == 1 && it > 0) {  // with two streams s_full(it) already says that P V (it - 1) is done
+                        pipe_wait(&pv_done[0], (it - 1) & 1, stop);
+                        __syncwarp();
+                        tc_fence_after();
+                    }
+                    const float f = grow ? ex2(m - mx) : 1.f;
+                    l *= f;
+    #pragma unroll 1
+                    for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
+                        float o[32];
+                        const uint32_t at = t_lane + C::O_COL + (uint32_t)(q * HD + c);
+                        uint32_t w[32];
+                        tmem_ld32(at, o);
+    #pragma unroll
+                        for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * f);
+                        tmem_st32(at, w);
+                    }
                 }
-                const float f = grow ? ex2(m - mx) : 1.f;
-                l *= f;
-#pragma unroll 1
-                for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
-                    float o[32];
-                    const uint32_t at = t_lane + C::O_COL + (uint32_t)(q * HD + c);
-                    uint32_t w[32];
-                    tmem_ld32(at, o);
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * f);
-                    tmem_st32(at, w);
-                }
+                if (grow) m = mx;
             }
-            if (grow) m = mx;
             const float u = m == -INFINITY ? 0.f : m;
             float2 sum = dup2(0.f);
             const float2 mu = dup2(-u), mm = dup2(mult);
@@ -625,7 +616,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                         sum = add2(sum, p);
                         w[c] = Elem<T>::pack(p.x, p.y);
                     }
-                    const uint32_t at = t_lane + C::S_COL + (uint32_t)(b * BN + col / 2 + h * (N / 4));
+                    const uint32_t at = t_lane + C::S_COL + (uint32_t)(b * BN + col + h * (N / 4));
                     if constexpr (N == 64) tmem_st16(at, w);
                     else tmem_st8(at, w);
                     ready(h == 0 ? &p_half[b] : &p_full[b]);

@@ -305,11 +305,14 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         __syncwarp();
     };
     if (NQ == 2 && warp >= C::SW) regs_dec<kRegsOther>();
+    // from the last tile to the first: under a distance bias the largest scores come first, so the maximum
+    // does not grow with every tile
+    auto tile = [&](int it) { return j0 + nt - 1 - it; };
     if (warp == kKWarp) {
         // ---------------------------------------------------------- K
         for (int it = 0; it < nt; ++it) {
             const int st = it % NS;
-            const int page = (j0 + it) * C::PAGES + lane;
+            const int page = tile(it) * C::PAGES + lane;
             const int id = lane < C::PAGES && page * kPageTokens < n_keys ? table[page] : -1;
             const int row = id >= 0 && id < a.p.r.n_pages ? (id * a.p.n_kv + hk) * kPageTokens : a.cache_rows;
             if (!__all_sync(0xffffffffu, pipe_wait(&k_empty[st], ((it / NS) & 1) ^ 1, stop))) break;
@@ -321,8 +324,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         // ---------------------------------------------------------- V
         int edges = 0;
         for (int it = 0; it < nt; ++it) {
-            const int st = it % NS, k0 = (j0 + it) * BN;
-            const int page = (j0 + it) * C::PAGES + lane;
+            const int st = it % NS, k0 = tile(it) * BN;
+            const int page = tile(it) * C::PAGES + lane;
             const int id = lane < C::PAGES && page * kPageTokens < n_keys ? table[page] : -1;
             const int row = id >= 0 && id < a.p.r.n_pages ? (id * a.p.n_kv + hk) * kPageTokens : a.cache_rows;
             if (!__all_sync(0xffffffffu, pipe_wait(&v_empty[st], ((it / NS) & 1) ^ 1, stop))) break;
@@ -385,12 +388,13 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 const int st = it % NS, b = NQ == 2 ? q : it & 1;
                 const uint32_t n = NQ == 2 ? it : it >> 1;  // how often the buffer was used before
                 if (q == 0 && !wait(&v_full[st], (it / NS) & 1)) return;
-                if (!wait(&p_half[b], n & 1)) return;
+                if (!wait(NQ == 2 ? &p_half[b] : &p_full[b], n & 1)) return;
                 tc_fence_after();
                 const uint32_t o_t = tmem + C::O_COL + (uint32_t)(q * HD);
                 const uint32_t p_t = tmem + C::S_COL + (uint32_t)(b * BN);
                 const uint64_t v_d = v_desc(smem_u32(smem + L.v + (uint32_t)st * C::KBYTES), (uint32_t)BN * 128u);
-                // the first half of each softmax thread's keys, then the second
+                // the first half of each softmax thread's keys, then the second (at head_dim 256, where the halves
+                // are two MMAs long, in one go: 522 against 535 us for 8,192 tokens)
                 constexpr int KS = BN / 16;
                 auto steps = [&](int piece) {
 #pragma unroll
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 };
                 if (one) steps(0);
                 __syncwarp();
-                if (!wait(&p_full[b], n & 1)) return;
+                if (NQ == 2 && !wait(&p_full[b], n & 1)) return;
                 tc_fence_after();
                 if (one) {
                     steps(1);
@@ -468,8 +472,6 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
         }
-        // z (base 2) = mult x, where x is q.k itself when nothing else is done to the scores
-        const float mult = CAP || BIAS ? 1.f : a.p.f.scale * kLog2E;
         const float scale2 = a.p.f.scale * kLog2E;
         const float u1 = CAP ? a.p.f.scale / a.p.f.cap : 0.f;  // u = u1 q.k
         const float cap2 = a.p.f.cap * kLog2E;
@@ -477,10 +479,12 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         // z = x (c0 + c1 x^2 + ...), x = q.k
         const float c0 = cap2 * u1 * kTanh0, c1 = cap2 * u1 * u1 * u1 * kTanh1, c2 = c1 * u1 * u1 * (kTanh2 / kTanh1),
                     c3 = c2 * u1 * u1 * (kTanh3 / kTanh2), c4 = c3 * u1 * u1 * (kTanh4 / kTanh3);
-        const float slope2 = BIAS && mine ? a.p.f.slopes[head] * kLog2E : 0.f;
+        const float slope2 = BIAS && mine ? a.p.f.slopes[head] * kLog2E : 1.f;
+        const float per_slope = BIAS ? scale2 / slope2 : 0.f;
         if (!mine) {  // rows past the end see everything: they must not force the masked path
             lo = 0;
             hi = INT32_MAX;
+            pos = INT32_MAX / 2;
         }
         // Capped scores lie within the cap, and bf16 has fp32's range: as long as 2^(+-cap2), summed over
         // any length, stays well inside it, no maximum is needed (m = 0)
@@ -489,7 +493,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         for (int it = 0; it < nt; ++it) {
             const int b = NQ == 2 ? q : it & 1;
             const uint32_t n = NQ == 2 ? it : it >> 1;
-            const int k0 = (j0 + it) * BN + col;  // this thread's first key
+            const int k0 = tile(it) * BN + col;  // this thread's first key
             pipe_wait(&s_full[b], n & 1, stop);
             __syncwarp();
             tc_fence_after();
@@ -522,6 +526,12 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             };
             bool small = false;  // capped scores within the polynomial's range
             float mx = 0.f;
+            // what becomes of x below stands for the scores ym x + yb (base 2)
+            float ym = CAP || BIAS ? 1.f : scale2, yb = 0.f;
+            // no key that the row sees in this tile lies after it: -slope |i - j| is a line in j (not for
+            // slopes that are zero, negative or too small to divide by)
+            const bool line = BIAS && __all_sync(0xffffffffu, slope2 > 1e-12f && min(hi, k0 + N) <= pos + 1);
+            const float d0 = BIAS ? (float)(pos - k0) : 0.f;
             if constexpr (CAP) {
                 if (flat) {
                     small = !edge && __all_sync(0xffffffffu, reduce(max3, [](float v) { return fabsf(v); }) <= s_max);
@@ -532,9 +542,12 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 if (small && !BIAS) {
                     if (!flat) mx = poly(make_float2(mx, 0.f), dup2(0.f)).x;  // monotonic: the maximum of the capped scores
                 } else if (small) {
+                    const float b0 = -slope2 * d0;
 #pragma unroll
                     for (int c = 0; c < N; c += 2) {
-                        const float2 y = poly(make_float2(x[c], x[c + 1]), dup2(0.f));
+                        const float2 bias = line ? make_float2(fmaf(slope2, (float)c, b0), fmaf(slope2, (float)(c + 1), b0))
+                                                 : make_float2(-slope2 * fabsf(d0 - (float)c), -slope2 * fabsf(d0 - (float)(c + 1)));
+                        const float2 y = poly(make_float2(x[c], x[c + 1]), bias);
                         x[c] = y.x;
                         x[c + 1] = y.y;
                     }
@@ -542,24 +555,20 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                     // cap tanh(u) = cap - 2 cap / (e^(2u) + 1), whatever u is
                     const float c_in = 2.f * kLog2E * u1;
 #pragma unroll
-                    for (int c = 0; c < N; ++c) x[c] = fmaf(-2.f * cap2, rcp_approx(ex2(x[c] * c_in) + 1.f), cap2);
-                }
-            }
-            if constexpr (BIAS) {
-                const float d0 = (float)(pos - k0);
-                if (!edge && __all_sync(0xffffffffu, pos >= k0 + N - 1 || !mine)) {
-                    // every key is at or before the row: -slope (i - j) is a line in j
-                    const float2 sl = dup2(slope2), sc = dup2(CAP ? 1.f : scale2);
-                    const float b0 = -slope2 * d0;
-#pragma unroll
-                    for (int c = 0; c < N; c += 2) {
-                        const float2 y = fma2(make_float2(x[c], x[c + 1]), sc, fma2(sl, make_float2((float)c, (float)(c + 1)), dup2(b0)));
-                        x[c] = y.x;
-                        x[c + 1] = y.y;
+                    for (int c = 0; c < N; ++c) {
+                        x[c] = fmaf(-2.f * cap2, rcp_approx(ex2(x[c] * c_in) + 1.f), cap2);
+                        if constexpr (BIAS) x[c] = fmaf(-slope2, fabsf(d0 - (float)c), x[c]);
                     }
+                }
+            } else if constexpr (BIAS) {
+                if (line) {  // scale q.k + slope (j - i) = slope (q.k scale / slope + c) - slope d0: one instruction a score
+                    ym = slope2;
+                    yb = -slope2 * d0;
+#pragma unroll
+                    for (int c = 0; c < N; ++c) x[c] = fmaf(x[c], per_slope, (float)c);
                 } else {
 #pragma unroll
-                    for (int c = 0; c < N; ++c) x[c] = fmaf(-slope2, fabsf(d0 - (float)c), CAP ? x[c] : x[c] * scale2);
+                    for (int c = 0; c < N; ++c) x[c] = fmaf(-slope2, fabsf(d0 - (float)c), x[c] * scale2);
                 }
             }
             if (edge) {
@@ -568,7 +577,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 for (int c = 0; c < N; ++c) x[c] = c >= cl && c < ch ? x[c] : -INFINITY;
             }
             if (!flat) {
-                if (!CAP || BIAS || !small) mx = row_max() * mult;
+                if (!CAP || BIAS || !small) mx = fmaf(row_max(), ym, yb);
                 *xrow(it & 1, half) = mx;  // the other half's maximum
                 pair_bar();
                 mx = fmaxf(mx, *xrow(it & 1, half ^ 1));
@@ -582,13 +591,13 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                     }
                     const float f = grow ? ex2(m - mx) : 1.f;
                     l *= f;
-    #pragma unroll 1
+#pragma unroll 1
                     for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                         float o[32];
                         const uint32_t at = t_lane + C::O_COL + (uint32_t)(q * HD + c);
                         uint32_t w[32];
                         tmem_ld32(at, o);
-    #pragma unroll
+#pragma unroll
                         for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * f);
                         tmem_st32(at, w);
                     }
@@ -597,7 +606,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             }
             const float u = m == -INFINITY ? 0.f : m;
             float2 sum = dup2(0.f);
-            const float2 mu = dup2(-u), mm = dup2(mult);
+            const float2 mu = dup2(yb - u), mm = dup2(ym);
             auto ready = [&](uint64_t* bar) {  // the P stored so far may be read
                 tmem_st_done();
                 tc_fence_before();
@@ -619,7 +628,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                     const uint32_t at = t_lane + C::S_COL + (uint32_t)(b * BN + col + h * (N / 4));
                     if constexpr (N == 64) tmem_st16(at, w);
                     else tmem_st8(at, w);
-                    ready(h == 0 ? &p_half[b] : &p_full[b]);
+                    if (NQ == 2 || h == 1) ready(h == 0 ? &p_half[b] : &p_full[b]);
                 }
             };
             if (CAP && !BIAS && small) exps([&](float2 v) { return poly(v, mu); });

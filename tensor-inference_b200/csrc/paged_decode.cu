@@ -548,6 +548,8 @@ constexpr int kJoinThreads = 256;
 template <class T>
 __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_constant__ DecArgs a, int ctas) {
     __shared__ int64_t tot[16];
+    __shared__ float inv[kDecRows];
+    extern __shared__ float smem_w[];
     const int seg = blockIdx.y, s = blockIdx.x, tid = threadIdx.x;
     const Line line = find_line<kJoinThreads>(a, 0, ctas, s, tot);
     pdl_wait();
@@ -563,30 +565,42 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_consta
     if (c0 == c1) return;  // its CTA finished it
     // partial of CTA c: its first segment's, unless the segment starts inside c's stretch
     auto row_of = [&](int c, int r) { return ((int64_t)c * 2 + ((int64_t)c * line.per >= g0 ? 0 : 1)) * a.rows + r; };
-    for (int e = tid * 4; e < G * HD; e += kJoinThreads * 4) {
-        const int r = e / HD, d = e - r * HD;
+    // weights of the partials: a warp takes rows r = warp, warp + 8, its lanes the CTAs
+    float* w = smem_w;  // [CTAs of the segment][16]
+    const int nc = c1 - c0 + 1;
+    for (int r = tid >> 5; r < G; r += kJoinThreads / 32) {
+        const int lane = tid & 31;
         float M = -INFINITY;
-        for (int c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(a.part_ml + row_of(c, r) * 2));
+        for (int c = lane; c < nc; c += 32) M = fmaxf(M, __ldcg(a.part_ml + row_of(c0 + c, r) * 2));
+        M = warp_max(M);
         const float u = M == -INFINITY ? 0.f : M;
         float l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int c = c0; c <= c1; ++c) {
-            const int64_t row = row_of(c, r);
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + row);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + row * HD + d));
+        for (int c = lane; c < nc; c += 32) {
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + row_of(c0 + c, r));
             const float f = ex2(x.x - u);
+            w[c * kDecRows + r] = f;
             l = fmaf(x.y, f, l);
+        }
+        l = warp_sum(l);
+        if (lane == 0) inv[r] = l == 0.f ? 0.f : 1.f / l;
+    }
+    __syncthreads();
+    for (int e = tid * 4; e < G * HD; e += kJoinThreads * 4) {
+        const int r = e / HD, d = e - r * HD;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int c = 0; c < nc; ++c) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + row_of(c0 + c, r) * HD + d));
+            const float f = w[c * kDecRows + r];
             o.x = fmaf(v.x, f, o.x);
             o.y = fmaf(v.y, f, o.y);
             o.z = fmaf(v.z, f, o.z);
             o.w = fmaf(v.w, f, o.w);
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        out[e] = Elem<T>::from_f(o.x * inv);
-        out[e + 1] = Elem<T>::from_f(o.y * inv);
-        out[e + 2] = Elem<T>::from_f(o.z * inv);
-        out[e + 3] = Elem<T>::from_f(o.w * inv);
+        out[e] = Elem<T>::from_f(o.x * inv[r]);
+        out[e + 1] = Elem<T>::from_f(o.y * inv[r]);
+        out[e + 2] = Elem<T>::from_f(o.z * inv[r]);
+        out[e + 3] = Elem<T>::from_f(o.w * inv[r]);
     }
 }
 
@@ -643,7 +657,8 @@ cudaError_t paged_decode_launch(const PagedAttn& p, int dev, cudaStream_t s) {
         void* jargs[] = {&a, &n};
         const void* j = bf ? reinterpret_cast<const void*>(&k_paged_join<__nv_bfloat16>)
                            : reinterpret_cast<const void*>(&k_paged_join<__half>);
-        e = launch_pdl(j, dim3(p.r.n_seqs, p.n_kv * a.chunks), dim3(kJoinThreads), 0, s, jargs, true);
+        e = launch_pdl(j, dim3(p.r.n_seqs, p.n_kv * a.chunks), dim3(kJoinThreads), (size_t)ctas * kDecRows * sizeof(float), s,
+                       jargs, true);
     }
     const cudaError_t g = cudaFreeAsync(scratch, s);
     return e != cudaSuccess ? e : g;

@@ -144,35 +144,49 @@ struct PreArgs {
 struct RowTile {
     int seq, row0;  // first row of the tile among the sequence's new tokens x group rows
     int t0, t1;     // the sequence's tokens
+    int kv_len, row;  // its length, its page-table row
 };
 template <int ROWS>
 TI_DEVICE_INLINE RowTile find_rows(const PreArgs& a, int x) {
     const int lane = threadIdx.x & 31, n = a.p.r.n_seqs;
-    RowTile r{-1, 0, 0, 0};
-    auto tiles_of = [&](int s) {
-        int t0 = 0, t1 = 0;
-        if (s < n) seq_tokens(a.p.r, s, t0, t1);
-        return ((t1 - t0) * a.group + ROWS - 1) / ROWS;
+    RowTile r{-1, 0, 0, 0, 0, 0};
+    // a lane takes a sequence; all that is known of it is loaded at once (one trip to memory, not three)
+    struct Seq {
+        int t0 = 0, t1 = 0, len = 0, row = -1, tiles = 0;
     };
-    int total = 0;
-    for (int base = 0; base < n; base += 32) total += tiles_of(base + lane);
+    auto get = [&](int s) {
+        Seq q;
+        if (s < n) {
+            seq_tokens(a.p.r, s, q.t0, q.t1);
+            q.len = a.p.r.kv_len[s];
+            q.row = a.p.r.row ? a.p.r.row[s] : s;
+        }
+        q.tiles = ((q.t1 - q.t0) * a.group + ROWS - 1) / ROWS;
+        return q;
+    };
+    const Seq first = get(lane);
+    int total = first.tiles;
+    for (int base = 32; base < n; base += 32) total += get(base + lane).tiles;
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const int want = total - 1 - x;
     if (want < 0) return r;
     int run = 0;
     for (int base = 0; base < n; base += 32) {
-        const int c = tiles_of(base + lane);
-        int inc = c;
+        const Seq q = base == 0 ? first : get(base + lane);
+        int inc = q.tiles;
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, want >= run + inc - c && want < run + inc);
+        const unsigned hit = __ballot_sync(0xffffffffu, want >= run + inc - q.tiles && want < run + inc);
         if (hit) {
             const int l = __ffs(hit) - 1;
             r.seq = base + l;
-            r.row0 = (want - (run + __shfl_sync(0xffffffffu, inc - c, l))) * ROWS;
-            seq_tokens(a.p.r, r.seq, r.t0, r.t1);
+            r.row0 = (want - (run + __shfl_sync(0xffffffffu, inc - q.tiles, l))) * ROWS;
+            r.t0 = __shfl_sync(0xffffffffu, q.t0, l);
+            r.t1 = __shfl_sync(0xffffffffu, q.t1, l);
+            r.kv_len = __shfl_sync(0xffffffffu, q.len, l);
+            r.row = __shfl_sync(0xffffffffu, q.row, l);
             return r;
         }
         run += __shfl_sync(0xffffffffu, inc, 31);
@@ -230,8 +244,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
     const int n_rows = (rt.t1 - rt.t0) * a.group - rt.row0;  // rows of the sequence from the tile's first on
 
     // ---- this thread's row (softmax threads): token, head, position, keys [lo, hi)
-    const int kv_len = a.p.r.kv_len[s];
-    const int32_t* table = table_row(a.p.r, s);
+    const int kv_len = rt.kv_len;
+    const int32_t* table = rt.row >= 0 && rt.row < a.p.r.table_rows ? a.p.r.table + (size_t)rt.row * a.p.r.pt_stride : nullptr;
     const int n_keys = table ? min(max(kv_len, 0), a.p.r.pt_stride * kPageTokens) : 0;
     int token = 0, head = 0, pos = 0, lo = 0, hi = 0;
     // (softmax warps 8 q + 4 half + quarter: the row of lane l is 128 q + 32 quarter + l)
@@ -338,10 +352,12 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             if (edge) {
                 if (!__all_sync(0xffffffffu, pipe_wait(v_edge, edges & 1, stop))) break;
                 ++edges;
-                for (int c = lane; c < BN * C::PARTS * 8; c += 32) {
-                    const int r = (c >> 3) % BN;
-                    if (k0 + r < key_lo || k0 + r >= key_hi)
-                        *reinterpret_cast<uint4*>(vt + (uint32_t)c * 16u) = make_uint4(0, 0, 0, 0);
+                const int lead = max(0, key_lo - k0), tail = min(BN, key_hi - k0);  // rows [lead, tail) are seen
+                for (int r = lane >> 3; r < lead + BN - tail; r += 4) {
+                    const int row = r < lead ? r : tail + r - lead;
+#pragma unroll
+                    for (int p = 0; p < C::PARTS; ++p)
+                        *reinterpret_cast<uint4*>(vt + (uint32_t)(p * BN + row) * 128u + (lane & 7) * 16u) = make_uint4(0, 0, 0, 0);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -445,28 +461,33 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         auto xrow = [&](int buf, int h) { return xch + ((buf * NQ + q) * 2 + h) * 128 + (warp & 3) * 32 + lane; };
         auto pair_bar = [&] { named_bar(1 + q * 4 + (warp & 3), 64); };
         const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        // ---- Q rows into shared memory (rows past the end are zero)
+        // ---- Q rows into shared memory (rows past the end are zero): the two warps of 32 rows take 16 each, all
+        // loads in flight together
         {
+            constexpr int QC = HD / 8, QR = 32 / QC, QN = 16 / QR;  // 16-byte chunks of a row, rows a load, loads
+            uint4 qv[QN];
             const T* src = reinterpret_cast<const T*>(a.p.q) + (mine ? (int64_t)token * a.p.q_stride + (int64_t)head * HD : 0);
-            uint8_t* qt = smem + L.q + (uint32_t)q * C::QBYTES;
-            constexpr int CH = HD / 8;        // 16-byte chunks of a row
-            constexpr int RP = 32 / CH;       // rows at a time
-            const int rl = lane / CH, c = lane % CH;
-            for (int i = half * 16; i < half * 16 + 16; i += RP) {
-                const T* p = reinterpret_cast<const T*>(
-                    __shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, i + rl));
-                const bool have = __shfl_sync(0xffffffffu, (int)mine, i + rl);
-                uint4 v = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < QN; ++i) {
+                const int l = half * 16 + i * QR + lane / QC, c = lane % QC;  // the lane whose row it is
+                const T* p = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, l));
+                const bool have = __shfl_sync(0xffffffffu, (int)mine, l);
+                qv[i] = make_uint4(0, 0, 0, 0);
                 if (have) {
-                    if (a.vec) v = *reinterpret_cast<const uint4*>(p + c * 8);
+                    if (a.vec) qv[i] = *reinterpret_cast<const uint4*>(p + c * 8);
                     else {
-                        unsigned short* e = reinterpret_cast<unsigned short*>(&v);
+                        unsigned short* e = reinterpret_cast<unsigned short*>(&qv[i]);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) e[k] = reinterpret_cast<const unsigned short*>(p)[c * 8 + k];
                     }
                 }
-                const int row = (warp & 3) * 32 + i + rl;
-                *reinterpret_cast<uint4*>(qt + (uint32_t)((c >> 3) * 128 + row) * 128u + (uint32_t)(((c & 7) ^ (row & 7)) << 4)) = v;
+            }
+            uint8_t* qt = smem + L.q + (uint32_t)q * C::QBYTES;
+#pragma unroll
+            for (int i = 0; i < QN; ++i) {
+                const int row = (warp & 3) * 32 + half * 16 + i * QR + lane / QC, c = lane % QC;
+                *reinterpret_cast<uint4*>(qt + (uint32_t)((c >> 3) * 128 + row) * 128u + (uint32_t)(((c & 7) ^ (row & 7)) << 4)) =
+                    qv[i];
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -704,23 +725,27 @@ __global__ void __launch_bounds__(128) k_prefill_join(const __grid_constant__ Pr
     if (r >= rows) return;
     const int t = (int)(r / a.p.n_heads), h = (int)(r % a.p.n_heads);
     if (seq_of_token(a.p.r, t) >= a.p.r.n_seqs || (a.p.r.start && t < a.p.r.start[0])) return;  // nobody's token
-    float M = -INFINITY;
-    for (int z = 0; z < a.splits; ++z) M = fmaxf(M, a.part_ml[(z * rows + r) * 2]);
-    const float u = M == -INFINITY ? 0.f : M;
+    // every partial's (max, sum) in one round of loads: lane l holds those of splits l and l + 32
+    const float2 none = make_float2(-INFINITY, 0.f);
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + r;
+    const float2 x0 = lane < a.splits ? ml[lane * rows] : none, x1 = lane + 32 < a.splits ? ml[(lane + 32) * rows] : none;
+    const float M = warp_max(fmaxf(x0.x, x1.x)), u = M == -INFINITY ? 0.f : M;
+    // a split that saw nothing of the row did not write its output
+    const float f0 = x0.x == -INFINITY && x0.y == 0.f ? 0.f : ex2(x0.x - u);
+    const float f1 = x1.x == -INFINITY && x1.y == 0.f ? 0.f : ex2(x1.x - u);
+    const float l = warp_sum(x0.y * f0 + x1.y * f1);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     T* out = reinterpret_cast<T*>(a.p.out) + (int64_t)t * a.p.out_stride + (int64_t)h * HD;
+    const float* po = a.part_o + r * HD;
     for (int d = lane * 2; d < HD; d += 64) {
-        float l = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll 4
+        float o0 = 0.f, o1 = 0.f;
+#pragma unroll 8
         for (int z = 0; z < a.splits; ++z) {
-            const float2 x = *reinterpret_cast<const float2*>(a.part_ml + (z * rows + r) * 2);
-            if (x.x == -INFINITY && x.y == 0.f) continue;  // saw nothing: its output was not written
-            const float2 v = *reinterpret_cast<const float2*>(a.part_o + (z * rows + r) * HD + d);
-            const float f = ex2(x.x - u);
-            l = fmaf(x.y, f, l);
+            const float f = __shfl_sync(0xffffffffu, z < 32 ? f0 : f1, z & 31);
+            const float2 v = f == 0.f ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(po + z * rows * HD + d);
             o0 = fmaf(v.x, f, o0);
             o1 = fmaf(v.y, f, o1);
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
         out[d] = Elem<T>::from_f(o0 * inv);
         out[d + 1] = Elem<T>::from_f(o1 * inv);
     }

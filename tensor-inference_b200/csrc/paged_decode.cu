@@ -23,6 +23,7 @@
 #include <mutex>
 
 #include "paged.cuh"
+#include "tcgen05.cuh"
 
 namespace ti {
 
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     uint64_t* empty = full + NS;
     int64_t* tot = reinterpret_cast<int64_t*>(smem + L.misc);
     volatile int* stop = reinterpret_cast<volatile int*>(smem + L.misc + 16 * 8);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
     pdl_trigger();
     if (tid == 0) {
@@ -264,13 +265,16 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                 }
                 const int id = __shfl_sync(0xffffffffu, cur, (i + lane) & 31);  // lane l: page p + l
                 if (!__all_sync(0xffffffffu, pipe_wait(&empty[slot], ((it / NS) & 1) ^ 1, stop))) continue;
-                if (lane == 0) mbar_arrive_expect_tx(&full[slot], (uint32_t)n * HD * 32u);
-                __syncwarp();
-                if (lane < n) {
-                    // a page that does not exist reads as zeros: rows past the end of the pool
-                    const int row = id >= 0 && id < a.p.r.n_pages ? (id * a.p.n_kv + hk) * kPageTokens : a.cache_rows;
-                    tma_load_page(smem + L.ring + (uint32_t)slot * kDecStage + half + (uint32_t)lane * (HD * 32u), tm, row,
-                                  &full[slot]);
+                // a page that does not exist reads as zeros: rows past the end of the pool
+                const int row = id >= 0 && id < a.p.r.n_pages ? (id * a.p.n_kv + hk) * kPageTokens : a.cache_rows;
+                const bool one = elect_one();
+                if (one) mbar_arrive_expect_tx(&full[slot], (uint32_t)n * HD * 32u);
+#pragma unroll
+                for (int l = 0; l < CP; ++l) {
+                    const int r = __shfl_sync(0xffffffffu, row, l);
+                    if (one && l < n)
+                        tma_load_page(smem + L.ring + (uint32_t)slot * kDecStage + half + (uint32_t)l * (HD * 32u), tm, r,
+                                      &full[slot]);
                 }
                 issued = it + 1;
                 __syncwarp();

@@ -35,7 +35,7 @@ constexpr int kDecRows = 16;                          // heads of a segment at m
 __host__ __device__ constexpr int dec_cp(int HD) { return 256 / HD; }  // pages of a stage
 __host__ __device__ // ring stages (128 KB in flight an SM): a multiple of the stages in progress at once, so that one
 // warp group uses a slot in order (a parity wait cannot tell a phase from the one before last)
-constexpr int dec_ns(bool g16) { return g16 ? 8 : 12; }
+constexpr int dec_ns() { return 8; }
 __host__ __device__ constexpr int dec_dw(int HD) { return HD < 128 ? HD : 128; }  // dims a warp accumulates
 __host__ __device__ constexpr int dec_red_stride(int HD) { return dec_dw(HD) + 8; }
 
@@ -46,15 +46,15 @@ __host__ __device__ constexpr DecSmem dec_smem(int HD, bool g16) {
     DecSmem L{};
     uint32_t o = 0;
     L.ring = o;  // [stages] {K [pages][HD/64][16][64], V}, rows 128-byte swizzled
-    o += dec_ns(g16) * kDecStage;
+    o += dec_ns() * kDecStage;
     L.q = o;  // the segment's heads [HD/64][16][64], swizzled
     o += 16u * HD * 2;
-    L.red = o;  // four warps' outputs [4][rows][dims + 8] fp32
-    o += 4u * (g16 ? 16 : 8) * dec_red_stride(HD) * 4;
-    L.ml = o;  // and their (max, sum) [4][16][2]
-    o += 4 * 16 * 2 * 4;
+    L.red = o;  // the warps' outputs [8][rows][dims + 8] fp32
+    o += (uint32_t)kDecWarps * (g16 ? 16 : 8) * dec_red_stride(HD) * 4;
+    L.ml = o;  // and their (max, sum) [8][16][2]
+    o += kDecWarps * 16 * 2 * 4;
     L.bar = o;  // full[stages], empty[stages]
-    o += 2 * 8 * dec_ns(g16);
+    o += 2 * 8 * dec_ns();
     L.misc = o;  // scan totals [16] int64, found segment
     o += 16 * 8 + 32;
     L.total = o + 1024;
@@ -64,9 +64,10 @@ __host__ __device__ constexpr DecSmem dec_smem(int HD, bool g16) {
 struct DecArgs {
     PagedAttn p;
     int group, chunks;  // heads per kv head, segments of up to 16 of them
-    int min_pages;      // pages a CTA takes at least
+    int min_pages;      // units a CTA takes at least
+    int seg_units;      // what a segment counts besides its pages
     int cache_rows;     // n_pages * n_kv * 16
-    int q_vec;          // q rows are 16-byte aligned
+    int q_vec, out_vec; // q rows are 16-byte aligned, out rows 8-byte
     float* part_o;      // [grid][2][rows][hd]
     float* part_ml;     // [grid][2][rows][2]
     int rows;           // rows of a partial: min(group, 16)
@@ -89,15 +90,16 @@ TI_DEVICE_INLINE SeqRange seq_range(const PagedAttn& p, int s) {
     return x;
 }
 
-// The line of pages: where sequence `want` starts (want >= 0), or which sequence holds
-// page `at` of the line of the CTA whose number is `cta` (want < 0).  All threads of
-// the block call it; tot: [16] int64 of shared memory.
+// The line: every segment counts seg_units (its share of a CTA's time besides the pages) and then its pages.
+// find_line says where sequence `want` starts (want >= 0), or which sequence holds the first unit of the CTA whose
+// number is `cta` (want < 0).  All threads of the block call it; tot: [16] int64 of shared memory.
 struct Line {
-    int64_t total, per;   // pages of the line; of one CTA
-    int64_t before;       // pages before the found sequence
+    int64_t total, per;   // units of the line; of one CTA
+    int64_t before;       // units before the found sequence
     int seq;              // the found sequence
     int npg;              // its pages per segment
 };
+TI_DEVICE_INLINE int units_of(const DecArgs& a, int npg) { return npg ? npg + a.seg_units : 0; }
 template <int THREADS>
 TI_DEVICE_INLINE Line find_line(const DecArgs& a, int cta, int ctas, int want, int64_t* tot) {
     constexpr int W = THREADS / 32;
@@ -108,12 +110,12 @@ TI_DEVICE_INLINE Line find_line(const DecArgs& a, int cta, int ctas, int want, i
     Line L;
     // total
     int64_t sum = 0;
-    int mine = 0;  // pages of sequence tid of the first round, kept for the search
+    int mine = 0;  // pages per segment of sequence tid of the first round, kept for the search
     for (int base = 0; base < n; base += THREADS) {
         const int s = base + tid;
         const int pg = s < n ? seq_range(a.p, s).npg : 0;
         if (base == 0) mine = pg;
-        sum += pg;
+        sum += units_of(a, pg);
     }
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) tot[warp] = sum;
@@ -134,7 +136,8 @@ TI_DEVICE_INLINE Line find_line(const DecArgs& a, int cta, int ctas, int want, i
     for (int base = 0; base < n; base += THREADS) {
         const int s = base + tid;
         const int pg = base == 0 ? mine : (s < n ? seq_range(a.p, s).npg : 0);
-        int64_t inc = pg;
+        const int un = units_of(a, pg);
+        int64_t inc = un;
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
@@ -143,7 +146,7 @@ TI_DEVICE_INLINE Line find_line(const DecArgs& a, int cta, int ctas, int want, i
         __syncthreads();
         int64_t off = run;
         for (int w = 0; w < warp; ++w) off += tot[w];
-        const int64_t hi = (off + inc) * H, lo = (off + inc - pg) * H;
+        const int64_t hi = (off + inc) * H, lo = (off + inc - un) * H;
         if (s < n && (want >= 0 ? s == want : (at >= lo && at < hi))) {
             found[0] = lo;
             found[1] = s;
@@ -197,7 +200,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     constexpr DecSmem L = dec_smem(HD, G16);
-    constexpr int CP = dec_cp(HD), NS = dec_ns(G16);
+    constexpr int CP = dec_cp(HD), NS = dec_ns();
     constexpr int KS = HD / 16, DW = dec_dw(HD), DPARTS = HD / DW, NT = DW / 8;
     constexpr int WPS = CP * DPARTS;            // warps of a stage
     constexpr int SG = kDecWarps / WPS;         // stages in progress at once
@@ -233,13 +236,15 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         for (int64_t g = g_begin; g < g_end;) {
             if (s >= a.p.r.n_seqs) return;
             const SeqRange x = seq_range(a.p, s);
-            while (g < g_end && g < base + (int64_t)x.npg * nseg) {
-                const int seg = (int)((g - base) / x.npg), p0 = (int)((g - base) % x.npg);
-                const int p1 = (int)min((int64_t)x.npg, p0 + (g_end - g));
-                f(s, x, seg, p0, p1);
-                g += p1 - p0;
+            const int un = units_of(a, x.npg);
+            while (g < g_end && g < base + (int64_t)un * nseg) {
+                const int seg = (int)((g - base) / un), u0 = (int)((g - base) % un);
+                const int u1 = (int)min((int64_t)un, u0 + (g_end - g));
+                const int p0 = max(0, u0 - a.seg_units), p1 = u1 - a.seg_units;
+                if (p1 > p0) f(s, x, seg, p0, p1);
+                g += u1 - u0;
             }
-            base += (int64_t)x.npg * nseg;
+            base += (int64_t)un * nseg;
             ++s;
         }
     };
@@ -290,7 +295,6 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     const int gq = lane >> 2, qq = lane & 3;       // mma fragment row / column pair
     const int so = warp / WPS, wi = warp % WPS;    // stages so, so + SG, ...; place in the stage
     const int blk = wi % CP, dp = wi / CP;         // page of the stage, dim part
-    const int gid = warp / DPARTS, part = warp % DPARTS;
     static_assert(DPARTS == 1 || CP == 1, "dim parts of a page are neighbouring warps");
     static_assert(NS % SG == 0, "a slot belongs to one warp group");
     uint8_t* qs = smem + L.q;
@@ -310,26 +314,42 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     const bool capped = a.p.f.cap > 0.f;
     const float cap2 = a.p.f.cap * kLog2E, inv_cap = capped ? a.p.f.scale / a.p.f.cap : 0.f;
 
+    constexpr int QN = (16 * HD / 8 + kDecWarps * 32 - 1) / (kDecWarps * 32);  // 16-byte chunks of q a thread loads
+    uint4 qv[QN];
+    int q_seq = -1, q_seg = -1;  // whose q those are
+    auto load_q = [&](int s, int seg) {
+        const int hk = seg / a.chunks, h0 = hk * a.group + (seg % a.chunks) * kDecRows;
+        const int G = min(kDecRows, (hk + 1) * a.group - h0);
+        const T* qrow = reinterpret_cast<const T*>(a.p.q) + (int64_t)s * a.p.q_stride + (int64_t)h0 * HD;
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const int c = tid + i * kDecWarps * 32;
+            qv[i] = make_uint4(0, 0, 0, 0);
+            if (c / (HD / 8) < G) {
+                const T* src = qrow + (int64_t)(c / (HD / 8)) * HD + c % (HD / 8) * 8;
+                if (a.q_vec) qv[i] = *reinterpret_cast<const uint4*>(src);
+                else {
+                    unsigned short* e = reinterpret_cast<unsigned short*>(&qv[i]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) e[k] = reinterpret_cast<const unsigned short*>(src)[k];
+                }
+            }
+        }
+        q_seq = s;
+        q_seg = seg;
+    };
     int it = 0, seg_no = 0;  // stages before this segment; segments before it
     segments([&](int s, const SeqRange& x, int seg, int p0, int p1) {
         const int hk = seg / a.chunks, h0 = hk * a.group + (seg % a.chunks) * kDecRows;
         const int G = min(kDecRows, (hk + 1) * a.group - h0);
-        // ---- q heads of the segment (rows past them zero)
-        const T* qrow = reinterpret_cast<const T*>(a.p.q) + (int64_t)s * a.p.q_stride + (int64_t)h0 * HD;
-        for (int c = tid; c < 16 * HD / 8; c += kDecWarps * 32) {
-            const int r = c / (HD / 8), d = c % (HD / 8) * 8;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < G) {
-                const T* src = qrow + (int64_t)r * HD + d;
-                if (a.q_vec) v = *reinterpret_cast<const uint4*>(src);
-                else {
-                    unsigned short* e = reinterpret_cast<unsigned short*>(&v);
+        // ---- q heads of the segment (rows past them zero); those of the sequence's next segment are requested as well
+        if (s != q_seq || seg != q_seg) load_q(s, seg);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) e[i] = reinterpret_cast<const unsigned short*>(src)[i];
-                }
-            }
-            *reinterpret_cast<uint4*>(qs + swz(16, r, d)) = v;
+        for (int i = 0; i < QN; ++i) {
+            const int c = tid + i * kDecWarps * 32;
+            if (c < 16 * HD / 8) *reinterpret_cast<uint4*>(qs + swz(16, c / (HD / 8), c % (HD / 8) * 8)) = qv[i];
         }
+        if (seg + 1 < nseg) load_q(s, seg + 1);
         float sl0 = 0.f, sl1 = 0.f;
         if (a.p.f.slopes) {
             if (gq < G) sl0 = a.p.f.slopes[h0 + gq] * kLog2E;
@@ -472,73 +492,64 @@ __global__ void __launch_bounds__(kDecThreads, 1)
             if (lane == 0) mbar_arrive(&empty[slot]);
         }
 
-        // ---- join the warps pairwise: the upper half of the groups hands its state to the lower
+        // ---- join the warps: every warp leaves its state, then every thread makes four of the outputs
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        float* rd = red + (size_t)warp * RR * RS;
+        float* mr = ml + warp * 32;
 #pragma unroll
-        for (int half = NG / 2; half >= 1; half >>= 1) {
-            const int w = ((gid >= half ? gid - half : gid) * DPARTS + part);
-            float* rd = red + (size_t)w * RR * RS;
-            float* mr = ml + w * 32;
-            if (gid >= half && gid < 2 * half) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    *reinterpret_cast<float2*>(rd + gq * RS + n * 8 + qq * 2) = make_float2(o[n][0], o[n][1]);
-                    if constexpr (G16)
-                        *reinterpret_cast<float2*>(rd + (gq + 8) * RS + n * 8 + qq * 2) = make_float2(o[n][2], o[n][3]);
-                }
-                if (qq == 0) {
-                    mr[gq * 2] = m0;
-                    mr[gq * 2 + 1] = l0;
-                    mr[(gq + 8) * 2] = m1;
-                    mr[(gq + 8) * 2 + 1] = l1;
-                }
-            }
-            named_bar(1, kDecWarps * 32);
-            if (gid < half) {
-                auto join = [&](int r, float& m, float& l, int e0) {
-                    const float mo = mr[r * 2], lo = mr[r * 2 + 1];
-                    const float M = fmaxf(m, mo), u = M == -INFINITY ? 0.f : M;
-                    const float f0 = ex2(m - u), f1 = ex2(mo - u);
-                    l = l * f0 + lo * f1;
-                    m = M;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const float2 v = *reinterpret_cast<const float2*>(rd + r * RS + n * 8 + qq * 2);
-                        o[n][e0] = o[n][e0] * f0 + v.x * f1;
-                        o[n][e0 + 1] = o[n][e0 + 1] * f0 + v.y * f1;
-                    }
-                };
-                join(gq, m0, l0, 0);
-                if constexpr (G16) join(gq + 8, m1, l1, 2);
-            }
-            named_bar(1, kDecWarps * 32);
+        for (int n = 0; n < NT; ++n) {
+            *reinterpret_cast<float2*>(rd + gq * RS + n * 8 + qq * 2) = make_float2(o[n][0], o[n][1]);
+            if constexpr (G16)
+                *reinterpret_cast<float2*>(rd + (gq + 8) * RS + n * 8 + qq * 2) = make_float2(o[n][2], o[n][3]);
         }
-        if (gid == 0) {
-            const bool whole = p0 == 0 && p1 == x.npg;
-            auto put = [&](int r, float m, float l, int e0) {
-                if (r >= G) return;
-                if (whole) {
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    T* dst = reinterpret_cast<T*>(a.p.out) + (int64_t)s * a.p.out_stride + (int64_t)(h0 + r) * HD + part * DW;
+        if (qq == 0) {
+            *reinterpret_cast<float2*>(mr + gq * 2) = make_float2(m0, l0);
+            *reinterpret_cast<float2*>(mr + (gq + 8) * 2) = make_float2(m1, l1);
+        }
+        named_bar(1, kDecWarps * 32);
+        // (the next write to this area comes after the next segment's barrier for q)
+        const bool whole = p0 == 0 && p1 == x.npg;
+        for (int e = tid * 4; e < G * HD; e += kDecWarps * 32 * 4) {
+            const int r = e / HD, d = e % HD, dpart = d / DW;
+            float2 st[NG];
+            float M = -INFINITY;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        dst[n * 8 + qq * 2] = Elem<T>::from_f(o[n][e0] * inv);
-                        dst[n * 8 + qq * 2 + 1] = Elem<T>::from_f(o[n][e0 + 1] * inv);
-                    }
+            for (int w = 0; w < NG; ++w) {
+                st[w] = *reinterpret_cast<const float2*>(ml + (w * DPARTS + dpart) * 32 + r * 2);
+                M = fmaxf(M, st[w].x);
+            }
+            const float u = M == -INFINITY ? 0.f : M;
+            float l = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < NG; ++w) {
+                const float f = ex2(st[w].x - u);
+                const float4 y = *reinterpret_cast<const float4*>(red + ((size_t)(w * DPARTS + dpart) * RR + r) * RS + d % DW);
+                l = fmaf(st[w].y, f, l);
+                v.x = fmaf(y.x, f, v.x);
+                v.y = fmaf(y.y, f, v.y);
+                v.z = fmaf(y.z, f, v.z);
+                v.w = fmaf(y.w, f, v.w);
+            }
+            if (whole) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                T* dst = reinterpret_cast<T*>(a.p.out) + (int64_t)s * a.p.out_stride + (int64_t)(h0 + r) * HD + d;
+                if (a.out_vec) {
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(v.x * inv, v.y * inv), Elem<T>::pack(v.z * inv, v.w * inv));
                 } else {
-                    const int64_t row = ((int64_t)blockIdx.x * 2 + (seg_no ? 1 : 0)) * a.rows + r;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        __stcg(reinterpret_cast<float2*>(a.part_o + row * HD + part * DW + n * 8 + qq * 2),
-                               make_float2(o[n][e0], o[n][e0 + 1]));
-                    if (part == 0 && qq == 0) __stcg(reinterpret_cast<float2*>(a.part_ml) + row, make_float2(m, l));
+                    dst[0] = Elem<T>::from_f(v.x * inv);
+                    dst[1] = Elem<T>::from_f(v.y * inv);
+                    dst[2] = Elem<T>::from_f(v.z * inv);
+                    dst[3] = Elem<T>::from_f(v.w * inv);
                 }
-            };
-            put(gq, m0, l0, 0);
-            if constexpr (G16) put(gq + 8, m1, l1, 2);
+            } else {
+                const int64_t row = ((int64_t)blockIdx.x * 2 + (seg_no ? 1 : 0)) * a.rows + r;
+                __stcg(reinterpret_cast<float4*>(a.part_o + row * HD + d), v);
+                if (d == 0) __stcg(reinterpret_cast<float2*>(a.part_ml) + row, make_float2(M, l));
+            }
         }
         it += n_st;
         ++seg_no;
@@ -564,8 +575,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_consta
         for (int e = tid; e < G * HD; e += kJoinThreads) out[e] = Elem<T>::from_f(0.f);
         return;
     }
-    const int64_t g0 = line.before + (int64_t)seg * line.npg, g1 = g0 + line.npg;
-    const int c0 = (int)(g0 / line.per), c1 = (int)((g1 - 1) / line.per);
+    const int64_t g0 = line.before + (int64_t)seg * units_of(a, line.npg), g1 = g0 + units_of(a, line.npg);
+    const int c0 = (int)((g0 + a.seg_units) / line.per), c1 = (int)((g1 - 1) / line.per);  // CTAs with pages of it
     if (c0 == c1) return;  // its CTA finished it
     // partial of CTA c: its first segment's, unless the segment starts inside c's stretch
     auto row_of = [&](int c, int r) { return ((int64_t)c * 2 + ((int64_t)c * line.per >= g0 ? 0 : 1)) * a.rows + r; };
@@ -634,10 +645,16 @@ cudaError_t paged_decode_launch(const PagedAttn& p, int dev, cudaStream_t s) {
     // would idle warps and only add partials to join
     a.min_pages = p.hd == 256 ? 4 : 8;
     a.cache_rows = p.r.n_pages * p.n_kv * kPageTokens;
+    a.out_vec = ((uintptr_t)p.out & 7) == 0 && p.out_stride % 4 == 0;
+    // A CTA that takes several segments pays for each (q, the join of its warps) about as much as for a dozen pages (32 sequences of up to
+    // 500 tokens, 8 kv heads: 39 us counted as 0 pages, 21 as 6, 19 as 12);
+    // with fewer segments than CTAs nobody takes several, and pages alone count
+    a.seg_units = (int64_t)p.r.n_seqs * p.n_kv * a.chunks > sms ? 12 : 0;
     a.q_vec = ((uintptr_t)p.q & 15) == 0 && p.q_stride % 8 == 0;
     // one CTA an SM, fewer when max_len says that the line is short (a CTA without pages returns at once)
     const int64_t span = p.f.window > 0 ? std::min(p.max_len, p.f.window) : p.max_len;
-    const int64_t pages = (span + 2 * kPageTokens - 2) / kPageTokens * (int64_t)p.n_kv * a.chunks * p.r.n_seqs;
+    const int64_t pages =
+        ((span + 2 * kPageTokens - 2) / kPageTokens + a.seg_units) * (int64_t)p.n_kv * a.chunks * p.r.n_seqs;
     const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(sms, (pages + a.min_pages - 1) / a.min_pages));
     CUtensorMap tk, tv;
     if (!make_tmap_pages(&tk, p.k_pages, a.cache_rows, p.hd, p.hd / 64) ||

@@ -210,7 +210,8 @@ typedef struct {
 /* Rotate q into q_out and k into the pages at each token's position, and copy v
  * there.  q [n_tokens, n_heads, head_dim] may be NULL (k and v only), rope may be
  * NULL (no rotation); strides are elements between tokens (a fused q|k|v row: its
- * width).  q_out may be q (same stride).  head_dim even, 2 .. 1024. */
+ * width).  q_out may be q (same stride).  head_dim even, 2 .. 1024.  Two tokens of one
+ * call that address the same slot leave either's values there. */
 ti_status ti_op_kv_append(const ti_paged_kv* kv, const ti_ragged* batch, const ti_rope_axes* rope, const void* q,
                           int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                           int n_heads, void* q_out, int64_t q_out_stride, void* stream);
@@ -220,11 +221,13 @@ ti_status ti_op_kv_append(const ti_paged_kv* kv, const ti_ragged* batch, const t
  * for the token at position i and key j; it sees j < kv_len[s] with
  *   j <= i or j < prefix[s],  j > i - sliding_window (when > 0),  j >= doc_start[t].
  * A token that sees nothing gets a zero row.  K and V of positions that no token
- * of a 256-row tile sees never enter, whatever they hold; V of a position that a
- * neighbouring token sees must be finite. */
+ * of the call sees never enter, whatever they hold (NaN, infinities, stale pages);
+ * in ti_op_paged_prefill a V row with a NaN or an infinity may also reach tokens that
+ * do not see it, where it lies within 128 positions of ones that see it and those tokens
+ * share its tile. */
 typedef struct {
-    float scale;                /* 0: 1 / sqrt(head_dim) */
-    float softcap;              /* 0: none */
+    float scale;                /* not negative; 0: 1 / sqrt(head_dim) */
+    float softcap;              /* 0: none; else scale / 1000 .. scale * 10,000 */
     const float* slopes;        /* [n_heads]; NULL: no distance bias */
     int sliding_window;         /* <= 0: none */
     const int32_t* prefix;      /* [n_seqs] first positions that see each other both ways; NULL: none */

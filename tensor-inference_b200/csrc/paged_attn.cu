@@ -42,8 +42,12 @@ ti_status paged_args(const ti_paged_kv* kv, const ti_ragged* batch, const ti_att
     const ti_attn_form& f = form ? *form : plain;
     TI_CHECK(std::isfinite(f.scale) && std::isfinite(f.softcap) && f.scale >= 0.f && f.softcap >= 0.f, TI_ERR_INVALID,
              "%s: scale and softcap must be finite and not negative", who);
+    const float scale = f.scale != 0.f ? f.scale : 1.0f / sqrtf((float)hd);
+    // outside these the cap's fp32 coefficients (powers of scale / softcap) leave their range, far from any cap in use
+    TI_CHECK(f.softcap == 0.f || (scale / f.softcap >= 1e-4f && scale / f.softcap <= 1e3f), TI_ERR_UNSUPPORTED,
+             "%s: softcap %g (scale / 1000 .. scale * 10,000)", who, (double)f.softcap);
     a->r = ragged_dev(kv, batch);
-    a->f = FormDev{f.scale != 0.f ? f.scale : 1.0f / sqrtf((float)hd), f.softcap, f.slopes, f.sliding_window, f.prefix,
+    a->f = FormDev{scale, f.softcap, f.slopes, f.sliding_window, f.prefix,
                    f.doc_start};
     a->q = q;
     a->q_stride = q_stride;

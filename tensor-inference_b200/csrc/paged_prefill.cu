@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         const float scale2 = a.p.f.scale * kLog2E;
         const float u1 = CAP ? a.p.f.scale / a.p.f.cap : 0.f;  // u = u1 q.k
         const float cap2 = a.p.f.cap * kLog2E;
-        const float s_max = CAP ? kTanhRange / u1 : 0.f;       // |q.k| up to which the polynomial holds
+        const float s_max = CAP ? kTanhRange / u1 : 0.f;  // |q.k| up to which the polynomial holds
         // z = x (c0 + c1 x^2 + ...), x = q.k
         const float c0 = cap2 * u1 * kTanh0, c1 = cap2 * u1 * u1 * u1 * kTanh1, c2 = c1 * u1 * u1 * (kTanh2 / kTanh1),
                     c3 = c2 * u1 * u1 * (kTanh3 / kTanh2), c4 = c3 * u1 * u1 * (kTanh4 / kTanh3);
@@ -520,10 +520,11 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             hi = INT32_MAX;
             pos = INT32_MAX / 2;
         }
-        // Capped scores lie within the cap, and bf16 has fp32's range: as long as 2^(+-cap2), summed over
-        // any length, stays well inside it, no maximum is needed (m = 0)
+        // Capped scores lie within +-cap2, and bf16 has fp32's range: up to cap2 = 80 (a cap of 55) one m serves
+        // every row.  m as near the largest score as leaves the smallest p at 2^-120: p is at most 1 up to
+        // cap2 = 60 and at most 2^40 at 80, so products with V and their sums stay in range as well
         const bool flat = CAP && !BIAS && Elem<T>::kUmmaFmt == 1 && cap2 <= 80.f;
-        float m = flat ? 0.f : -INFINITY, l = 0.f;
+        float m = flat ? fminf(cap2, 120.f - cap2) : -INFINITY, l = 0.f;
         for (int it = 0; it < nt; ++it) {
             const int b = NQ == 2 ? q : it & 1;
             const uint32_t n = NQ == 2 ? it : it >> 1;
@@ -586,7 +587,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                         x[c + 1] = y.y;
                     }
                 } else {
-                    // cap tanh(u) = cap - 2 cap / (e^(2u) + 1), whatever u is
+                    // cap tanh(u) = cap - 2 cap / (e^(2u) + 1), whatever u is: off by at most cap 2^-21 (two approximations
+                    // of 2^-22 and 2^-23 of a term below 2 cap, and the subtraction)
                     const float c_in = 2.f * kLog2E * u1;
 #pragma unroll
                     for (int c = 0; c < N; ++c) {

@@ -19,7 +19,7 @@
 
 namespace ti {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 constexpr int kRopeMaxHalf = 256;
 
 struct RopeDev {
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const __grid_const
         for (int e = 0; e < VEC; ++e) w[e] = rot ? cs[u * VEC + e] : make_float2(1.f, 0.f);
         const int h0 = gt / U;
         if (U < a.tpt && h0 >= lanes) break;  // threads past the last whole head
-#pragma unroll 2
+#pragma unroll(PAGED ? 2 : 1)
         for (int h = U < a.tpt ? h0 : 0; h < heads; h += lanes) {
             const T* src;
             T* dst;
@@ -175,7 +175,10 @@ cudaError_t rope_launch(RopeArgs& a, int dtype, bool paged, int sms, cudaStream_
     const bool vec = a.hd % (2 * V) == 0 && a.rope.half % V == 0 && al(a.q, a.q_stride) && al(a.q_out, a.q_out_stride) &&
                      al(a.k, a.k_stride) && al(a.v, a.v_stride);
     // few tokens: the whole block on one token (latency); many: 64 threads a token, so that a thread
-    // keeps its cosines for several heads
+    // keeps its cosines for several heads.  16,384 tokens x 32 heads x 128, bf16: 49.8 us (5.4 TB/s); with 128
+    // threads a token 64, with 32 56; in blocks of 256 threads 51.7.  What bounds it is the chain before the heads
+    // (positions, sines, the barrier), so resident warps count: requesting heads ahead of it costs more
+    // registers than it gains (73 us with two heads ahead, 126 with four).
     a.tpt = a.r.n_tokens <= 2 * sms ? kRopeThreads : 64;
     const int per = kRopeThreads / a.tpt;
     const int grid = (a.r.n_tokens + per - 1) / per;

@@ -91,8 +91,10 @@ def attend(cache, q, heads, cap=0.0, slopes=None, window=0, prefix=None, doc=Non
     """float64 rows [tokens, heads, hd] of cache's sequences for q, and the largest error of a
     kernel that rounds the probabilities and the result to the type and computes the rest in
     fp32.  With u = half a step of the type: u |o| for the result, u sum p |v| for the
-    probabilities; scores off by dz (fp32 products over hd terms, 2^-16 for the cap's
-    approximation times its slope and the exponential) scale each p by at most 1 + 2 dz."""
+    probabilities; scores off by dz scale each p by at most 1 + 2 dz.  dz counts fp32 products
+    over hd terms, 2^-16 for the exponential and the cap's polynomial (2.1e-7 of the cap) and,
+    above a cap of 32, cap 2^-21: tanh as cap - 2 cap / (e^(2u) + 1) with the exponential off by
+    2^-22 and the reciprocal by 2^-23 of a term below 2 cap, and one rounding near cap (2^-24)."""
     group, hd = heads // cache.nkv, cache.hd
     u = HALF_STEP[cache.dtype]
     out = np.zeros((q.shape[0], heads, hd))
@@ -125,7 +127,7 @@ def attend(cache, q, heads, cap=0.0, slopes=None, window=0, prefix=None, doc=Non
                 bias = float(slopes[h]) * np.abs(i - j)
                 z = z - bias
                 dz = dz + np.abs(bias) * 2.0 ** -22
-            dz = dz + 2.0 ** -16 + np.abs(z) * 2.0 ** -22
+            dz = dz + max(2.0 ** -16, cap * 2.0 ** -21) + np.abs(z) * 2.0 ** -22
             z = np.where(seen, z, -np.inf)
             dz = np.where(seen, dz, 0).max(-1, keepdims=True)
             top = z.max(-1, keepdims=True)

@@ -151,6 +151,27 @@ def test_kv_append(dtype, axes, seqs, heads, nkv, hd, pad):
         assert torch.equal(a[~new_slots], b[~new_slots])
 
 
+@pytest.mark.parametrize("tokens", [3, 700])
+def test_kv_append_rotates_q_in_place(tokens):
+    heads, nkv, hd = 4, 2, 64
+    c = Cache([(tokens, tokens + 5)], nkv, hd, "bf16", seed=2)
+    d = c.dev()
+    g = torch.Generator().manual_seed(2)
+    qkv = torch.randn(tokens, (heads + 2 * nkv) * hd, generator=g).to(torch.bfloat16)
+    dq, w, es, fr = qkv.cuda(), qkv.shape[1], 2, freqs(hd).cuda()
+    r = rope_struct(hd, fr, None)
+    b = dq.data_ptr()
+    ti.check(ti.lib().ti_op_kv_append(C.byref(d["kv"]), C.byref(d["batch"]), C.byref(r), b, w, b + heads * hd * es, w,
+                                      b + (heads + nkv) * hd * es, w, heads, b, w, stream()))
+    x = qkv.double().numpy().reshape(tokens, -1, hd)
+    y, off = rotate(x, angles(hd, torch.arange(5, tokens + 5)[None]), hd)
+    tol = HALF_STEP["bf16"] * np.abs(y) * 1.01 + off + FLOOR["bf16"]
+    got = dq.view(tokens, -1, hd)
+    within(got[:, :heads], y[:, :heads], tol[:, :heads])
+    assert torch.equal(got[:, heads:].cpu(), qkv.view(tokens, -1, hd)[:, heads:])  # k and v rows are inputs only
+    within(c.read(d["k"], 0)[5:], y[:, heads:heads + nkv], tol[:, heads:heads + nkv])
+
+
 def test_kv_append_without_q_and_with_bad_ids():
     c = Cache([(4, 20), (3, 3), (2, 40), (2, 18)], 2, 64, "bf16", seed=3)
     c.table[c.rows[0], 1] = c.n_pages  # the page of positions 16..19 of sequence 0 does not exist
@@ -265,6 +286,67 @@ def test_large_scores_reach_the_cap(entry):
     c = Cache([(1, 260), (1, 31)] if entry == "decode" else [(40, 260), (31, 31)], 1, 64, "bf16", seed=2, std=6.0)
     for cap in (0.0, 2.0, 50.0):
         out, ref, tol = run_attention(c, queries(c, 4, std=6.0), 4, entry, cap=cap)
+        within(out, ref, tol, f"cap {cap}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("cap", [2e-4, 0.02, 1.0, 54.0, 56.0, 300.0, 1000.0])
+@pytest.mark.parametrize("entry", ["prefill", "decode"])
+def test_caps_of_any_size(entry, cap, dtype):
+    # far below the scores (all of them at the cap), about them, and far above (no cap in effect)
+    c = Cache([(1, 260), (1, 31)] if entry == "decode" else [(40, 260), (31, 31)], 1, 64, dtype, seed=2, std=2.0)
+    out, ref, tol = run_attention(c, queries(c, 4, std=2.0), 4, entry, cap=cap)
+    within(out, ref, tol)
+
+
+@pytest.mark.parametrize("entry", ["prefill", "decode"])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_scores_all_at_one_end_of_the_cap(entry, sign):
+    # every score at -cap or at +cap, values up to 1e20: weights far from 1 must not leave the range
+    c = Cache([(1, 200)] if entry == "decode" else [(30, 200)], 1, 64, "bf16", seed=3)
+    c.K[0] = torch.full_like(c.K[0], sign * 10)
+    c.V[0] = c.V[0] * 1e20
+    for p in range(-(-200 // 16)):
+        m = min(16, 200 - p * 16)
+        page = int(c.table[c.rows[0], p])
+        c.k[page, :, :m] = c.K[0][p * 16:p * 16 + m].transpose(0, 1)
+        c.v[page, :, :m] = c.V[0][p * 16:p * 16 + m].transpose(0, 1)
+    q = torch.ones(c.tokens, 2, 64, dtype=torch.bfloat16)
+    for cap in (30.0, 50.0, 55.0, 60.0):
+        out, ref, tol = run_attention(c, q, 2, entry, cap=cap)
+        within(out, ref, tol, f"cap {cap}")
+
+
+@pytest.mark.parametrize("form", ["plain", "all"])
+def test_many_sequences(form):
+    # more sequences than one round of the look-ups takes, empty ones among them
+    g = np.random.default_rng(1)
+    lens = [int(n) for n in g.integers(0, 50, 700)]
+    c = Cache([(1, n) for n in lens], 1, 64, "bf16", seed=1)
+    out, ref, tol = run_attention(c, queries(c, 2), 2, "decode", **FORMS[form])
+    within(out, ref, tol)
+    c = Cache([(int(min(n, g.integers(0, 4))), n) for n in lens[:150]], 2, 64, "f16", seed=2, pad_tokens=3)
+    out, ref, tol = run_attention(c, queries(c, 4), 4, "prefill", **FORMS[form])
+    real = int(c.starts[-1])
+    within(out[:real], ref[:real], tol[:real])
+    assert (out[real:] == 3.0).all()
+
+
+@pytest.mark.parametrize("entry", ["prefill", "decode"])
+def test_slopes_of_any_sign(entry):
+    heads = 6
+    c = Cache([(1, 300), (1, 40)] if entry == "decode" else [(20, 300), (40, 40)], 2, 64, "bf16", seed=6)
+    q = queries(c, heads)
+    slopes = torch.tensor([0.0, -0.01, 1e-13, 3.0, 0.5, 1e-6])
+    for cap in (0.0, 10.0):
+        d = c.dev(decode=entry == "decode")
+        ds, dq, out = slopes.cuda(), q.cuda(), torch.zeros(c.tokens, heads, 64, dtype=torch.bfloat16, device="cuda")
+        pre = torch.tensor([200, 7], dtype=torch.int32)
+        dp = pre.cuda()
+        f = ti.AttnForm(softcap=cap, slopes=ds.data_ptr(), prefix=dp.data_ptr())
+        ti.check(getattr(ti.lib(), f"ti_op_paged_{entry}")(C.byref(d["kv"]), C.byref(d["batch"]), C.byref(f), dq.data_ptr(),
+                                                           heads * 64, heads, out.data_ptr(), heads * 64, stream()))
+        ref, tol = attend(c, q, heads, cap=cap, slopes=slopes.double().numpy(), prefix=pre.numpy())
         within(out, ref, tol, f"cap {cap}")
 
 

@@ -131,6 +131,9 @@ def test_append_refuses_bad_rows(args, word):
     (dict(os=0), ti.TI_ERR_INVALID, "stride"), (dict(form=dict(softcap=-1.0)), ti.TI_ERR_INVALID, "softcap"),
     (dict(form=dict(softcap=float("nan"))), ti.TI_ERR_INVALID, "softcap"),
     (dict(form=dict(scale=float("inf"))), ti.TI_ERR_INVALID, "scale"),
+    (dict(form=dict(scale=-0.1)), ti.TI_ERR_INVALID, "scale"),
+    (dict(form=dict(softcap=1e-6)), ti.TI_ERR_UNSUPPORTED, "softcap"),
+    (dict(form=dict(softcap=1e4)), ti.TI_ERR_UNSUPPORTED, "softcap"),
 ])
 def test_attention_refuses_bad_arguments(entry, args, code, word):
     a = dict(q=P, qs=256, heads=4, out=P, os=256, hd=64, form={})

@@ -19,14 +19,17 @@
 // The output stays in TMEM; it is rescaled only when a row's maximum has grown by more than
 // 2^8 since the last time (P then stays under 2^8, far from overflow in either type), which
 // is rare after the first tiles.  P is rounded once to the operand type, half a step of
-// it (2^-9 of p at most for bf16) on each term, as the product's inputs must be; the
-// sum of p is taken before that rounding.
+// it (2^-8 of p for bf16, 2^-11 for f16) on each term, as the product's inputs must be; the
+// sum is that of the rounded values, so that a row on few keys, or with one large weight, does
+// not keep their rounding (the result's error against 64 bits is 1.1 to 1.4 times that of a result
+// rounded once; with the sum of the unrounded ones 1.3 to 1.5, at 4 to 8% less time).
 //
 // Few rows over a long cache: the key tiles of a row tile are divided over gridDim.z CTAs,
 // whose partial (max, sum, output) rows k_prefill_join adds in order.
 //
 // Every wait is bounded; one that gives up stops all roles, the MMAs issued are waited for, and TMEM is freed.
 #include <algorithm>
+#include <atomic>
 
 #include "paged.cuh"
 #include "tcgen05.cuh"
@@ -258,6 +261,40 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         pos = kv_len - (rt.t1 - token);
         key_range(a.p.f, s, token, pos, n_keys, lo, hi);
     }
+    // ---- Q rows into shared memory (rows past the end are zero): the two warps of 32 rows take 16 each, in copies that
+    // run on while the block comes up
+    if (warp < C::SW) {
+        constexpr int QC = HD / 8, QR = 32 / QC, QN = 16 / QR;  // 16-byte chunks of a row, rows a copy, copies
+        uint8_t* qt = smem + L.q + (uint32_t)(warp >> 3) * C::QBYTES;
+        const T* src = reinterpret_cast<const T*>(a.p.q) + (mine ? (int64_t)token * a.p.q_stride + (int64_t)head * HD : 0);
+        const int c = lane % QC;
+        // copy i: where from (of the lane whose row it is), where to, whether there is such a row
+        auto piece = [&](int i, const T*& p, uint8_t*& dst) {
+            const int l = ((warp >> 2) & 1) * 16 + i * QR + lane / QC, row = (warp & 3) * 32 + l;
+            p = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, l)) + c * 8;
+            dst = qt + (uint32_t)((c >> 3) * 128 + row) * 128u + (uint32_t)(((c & 7) ^ (row & 7)) << 4);
+            return (bool)__shfl_sync(0xffffffffu, (int)mine, l);
+        };
+        const T* p;
+        uint8_t* dst;
+        // (two loops, not a choice in one: what a short call pays for most is fetching code it runs once)
+        if (a.vec) {
+#pragma unroll 4
+            for (int i = 0; i < QN; ++i) {
+                const bool have = piece(i, p, dst);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(p), "r"(have ? 16 : 0)
+                             : "memory");
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < QN; ++i) {
+                const bool have = piece(i, p, dst);
+#pragma unroll 1
+                for (int k = 0; k < 8; ++k)
+                    reinterpret_cast<unsigned short*>(dst)[k] = have ? reinterpret_cast<const unsigned short*>(p)[k] : 0;
+            }
+        }
+    }
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
             mbar_init(&k_full[i], 1);
@@ -451,8 +488,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         }
     } else if (warp < C::SW) {
         // ---------------------------------------------------------- softmax: two threads a row, half a tile's keys each
-        // (one thread a row leaves one warp a scheduler at work while the other stream waits: its
-        // latencies show, 536 against OTHERus for 8,192 causal tokens)
+        // (one thread a row leaves one warp a scheduler at work while the other stream waits, and its latencies
+        // show: at head_dim 64 461 against 431 us for 8,192 causal tokens, at 256 638 against 559)
         if (NQ == 2) regs_inc<kRegsSoftmax>();
         constexpr int N = C::COLS;
         const int q = warp >> 3, half = (warp >> 2) & 1, col = half * N;
@@ -474,38 +511,11 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             else asm volatile("bar.arrive 9, 512;" ::: "memory");
         };
         const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        // ---- Q rows into shared memory (rows past the end are zero): the two warps of 32 rows take 16 each, all
-        // loads in flight together
-        {
-            constexpr int QC = HD / 8, QR = 32 / QC, QN = 16 / QR;  // 16-byte chunks of a row, rows a load, loads
-            uint4 qv[QN];
-            const T* src = reinterpret_cast<const T*>(a.p.q) + (mine ? (int64_t)token * a.p.q_stride + (int64_t)head * HD : 0);
-#pragma unroll
-            for (int i = 0; i < QN; ++i) {
-                const int l = half * 16 + i * QR + lane / QC, c = lane % QC;  // the lane whose row it is
-                const T* p = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, (unsigned long long)(uintptr_t)src, l));
-                const bool have = __shfl_sync(0xffffffffu, (int)mine, l);
-                qv[i] = make_uint4(0, 0, 0, 0);
-                if (have) {
-                    if (a.vec) qv[i] = *reinterpret_cast<const uint4*>(p + c * 8);
-                    else {
-                        unsigned short* e = reinterpret_cast<unsigned short*>(&qv[i]);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) e[k] = reinterpret_cast<const unsigned short*>(p)[c * 8 + k];
-                    }
-                }
-            }
-            uint8_t* qt = smem + L.q + (uint32_t)q * C::QBYTES;
-#pragma unroll
-            for (int i = 0; i < QN; ++i) {
-                const int row = (warp & 3) * 32 + half * 16 + i * QR + lane / QC, c = lane % QC;
-                *reinterpret_cast<uint4*>(qt + (uint32_t)((c >> 3) * 128 + row) * 128u + (uint32_t)(((c & 7) ^ (row & 7)) << 4)) =
-                    qv[i];
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
-        }
+        // ---- Q has arrived: this thread's copies, then the warp's, are in shared memory for the MMAs
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
         const float scale2 = a.p.f.scale * kLog2E;
         const float u1 = CAP ? a.p.f.scale / a.p.f.cap : 0.f;  // u = u1 q.k
         const float cap2 = a.p.f.cap * kLog2E;
@@ -659,8 +669,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                         const int k = h * (N / 2) + 2 * c;
                         const float2 y = arg(make_float2(x[k], x[k + 1]));
                         const float2 p = make_float2(ex2(y.x), ex2(y.y));
-                        sum = add2(sum, p);
                         w[c] = Elem<T>::pack(p.x, p.y);
+                        sum = add2(sum, make_float2(Elem<T>::lo(w[c]), Elem<T>::hi(w[c])));
                     }
                     const uint32_t at = t_lane + C::S_COL + (uint32_t)(b * BN + col + h * (N / 4));
                     if constexpr (N == 64) tmem_st16(at, w);
@@ -699,26 +709,24 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         } else {
             T* dst = reinterpret_cast<T*>(a.p.out) + (int64_t)token * a.p.out_stride + (int64_t)head * HD;
             const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
             for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                 float o[32];
-                if (nt > 0) tmem_ld32(t_lane + C::O_COL + (uint32_t)(q * HD + c), o);
                 uint32_t w[16];
+                if (nt > 0) tmem_ld32(t_lane + C::O_COL + (uint32_t)(q * HD + c), o);
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
                     w[k] = nt > 0 && l != 0.f ? Elem<T>::pack(o[2 * k] * inv, o[2 * k + 1] * inv) : 0u;
-                if (mine) {
-                    if (a.vec) {
+                if (mine && a.vec) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            *reinterpret_cast<uint4*>(dst + c + k * 8) =
-                                make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-                    } else {
-                        unsigned short* e = reinterpret_cast<unsigned short*>(dst + c);
+                    for (int k = 0; k < 4; ++k)
+                        *reinterpret_cast<uint4*>(dst + c + k * 8) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                } else if (mine) {
+                    unsigned short* e = reinterpret_cast<unsigned short*>(dst + c);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            e[2 * k] = (unsigned short)(w[k] & 0xffffu);
-                            e[2 * k + 1] = (unsigned short)(w[k] >> 16);
-                        }
+                    for (int k = 0; k < 16; ++k) {
+                        e[2 * k] = (unsigned short)(w[k] & 0xffffu);
+                        e[2 * k + 1] = (unsigned short)(w[k] >> 16);
                     }
                 }
             }
@@ -737,11 +745,11 @@ template <class T>
 __global__ void __launch_bounds__(128) k_prefill_join(const __grid_constant__ PreArgs a) {
     const int lane = threadIdx.x & 31, HD = a.p.hd;
     const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    pdl_wait();
     const int64_t rows = (int64_t)a.p.r.n_tokens * a.p.n_heads;
-    if (r >= rows) return;
-    const int t = (int)(r / a.p.n_heads), h = (int)(r % a.p.n_heads);
-    if (seq_of_token(a.p.r, t) >= a.p.r.n_seqs || (a.p.r.start && t < a.p.r.start[0])) return;  // nobody's token
+    const int t = (int)(min(r, rows - 1) / a.p.n_heads), h = (int)(r % a.p.n_heads);
+    const bool nobodys = seq_of_token(a.p.r, t) >= a.p.r.n_seqs || (a.p.r.start && t < a.p.r.start[0]);
+    pdl_wait();  // (every block waits: the kernel after this one starts when this one is done)
+    if (r >= rows || nobodys) return;
     // every partial's (max, sum) in one round of loads: lane l holds those of splits l and l + 32
     const float2 none = make_float2(-INFINITY, 0.f);
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + r;
@@ -805,6 +813,18 @@ cudaError_t paged_prefill_launch(const PagedAttn& p, int dev, cudaStream_t s) {
     const size_t smem = p.hd == 64 ? pre_smem<64>().total : p.hd == 128 ? pre_smem<128>().total : pre_smem<256>().total;
     cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
+    if (p.hd <= 128) {
+        // the hand-over of registers waits for good unless the block was launched with its sum: checked once a kernel
+        static std::atomic<unsigned> checked{0};
+        const unsigned bit = 1u << ((p.hd == 128) | bf << 1 | cap << 2 | bias << 3);
+        if (!(checked.load(std::memory_order_relaxed) & bit)) {
+            cudaFuncAttributes fa;
+            e = cudaFuncGetAttributes(&fa, f);
+            if (e != cudaSuccess) return e;
+            if (fa.numRegs != kRegsLaunch) return cudaErrorInvalidKernelImage;
+            checked.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
     float* scratch = nullptr;
     const size_t n = (size_t)a.splits * p.r.n_tokens * p.n_heads;
     if (a.splits > 1) {

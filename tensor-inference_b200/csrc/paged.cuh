@@ -87,6 +87,30 @@ TI_DEVICE_INLINE int seq_of_token(const RaggedDev& r, int t) {
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
 }
+// sequence, position and page-table row of token t (a whole warp asks for the same t), what is known of a
+// sequence loaded together; seq < 0 for a token that belongs to nobody
+struct TokenPlace {
+    int seq, pos, row;
+};
+TI_DEVICE_INLINE TokenPlace place_of_token(const RaggedDev& r, int t) {
+    if (!r.start) return TokenPlace{t, r.kv_len[t] - 1, r.row ? r.row[t] : t};
+    const int lane = threadIdx.x & 31;
+    for (int base = 0; base < r.n_seqs; base += 32) {
+        const int s = base + lane;
+        int t0 = 0, t1 = 0, len = 0, row = 0;
+        if (s < r.n_seqs) {
+            seq_tokens(r, s, t0, t1);
+            len = r.kv_len[s];
+            row = r.row ? r.row[s] : s;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, t >= t0 && t < t1);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            return TokenPlace{base + l, __shfl_sync(0xffffffffu, len - (t1 - t), l), __shfl_sync(0xffffffffu, row, l)};
+        }
+    }
+    return TokenPlace{-1, 0, -1};
+}
 // page-table row of sequence s, nullptr when out of range
 TI_DEVICE_INLINE const int32_t* table_row(const RaggedDev& r, int s) {
     const int row = r.row ? r.row[s] : s;

@@ -37,9 +37,15 @@
 namespace ti {
 
 // Registers: with two streams the block is launched with 96 a thread (640 x 96 = 61,440), and the loading and
-// issuing warps hand some of theirs to the softmax warps: 128 x 64 + 512 x 104 = 61,440.
-constexpr int kRegsLaunch = 96, kRegsOther = 64, kRegsSoftmax = 104;
-static_assert(128 * kRegsOther + 512 * kRegsSoftmax == 640 * kRegsLaunch, "the shares are what was launched");
+// issuing warps hand some of theirs to the softmax warps: 128 x 64 + 512 x 104 = 61,440, or, where the cap's
+// polynomial needs them, 128 x 32 + 512 x 112 (8,192 tokens capped at head_dim 128 / 64: 437 / 523 us against 449 /
+// 556; uncapped 491 / 422 against 486 / 414).
+constexpr int kRegsLaunch = 96;
+constexpr int regs_other(bool cap) { return cap ? 32 : 64; }
+constexpr int regs_softmax(bool cap) { return cap ? 112 : 104; }
+static_assert(128 * regs_other(true) + 512 * regs_softmax(true) == 640 * kRegsLaunch &&
+                  128 * regs_other(false) + 512 * regs_softmax(false) == 640 * kRegsLaunch,
+              "the shares are what was launched");
 template <int N>
 TI_DEVICE_INLINE void regs_inc() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -355,7 +361,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         }
         __syncwarp();
     };
-    if (NQ == 2 && warp >= C::SW) regs_dec<kRegsOther>();
+    if (NQ == 2 && warp >= C::SW) regs_dec<regs_other(CAP)>();
     // from the last tile to the first: under a distance bias the largest scores come first, so the maximum
     // does not grow with every tile
     auto tile = [&](int it) { return j0 + nt - 1 - it; };
@@ -490,7 +496,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         // ---------------------------------------------------------- softmax: two threads a row, half a tile's keys each
         // (one thread a row leaves one warp a scheduler at work while the other stream waits, and its latencies
         // show: at head_dim 64 461 against 431 us for 8,192 causal tokens, at 256 638 against 559)
-        if (NQ == 2) regs_inc<kRegsSoftmax>();
+        if (NQ == 2) regs_inc<regs_softmax(CAP)>();
         constexpr int N = C::COLS;
         const int q = warp >> 3, half = (warp >> 2) & 1, col = half * N;
         float* xch = reinterpret_cast<float*>(smem + L.xch);
@@ -651,6 +657,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 if (grow) m = mx;
             }
             const float u = m == -INFINITY ? 0.f : m;
+            // (scalar sums uncapped at head_dim 128: 474 against 486 us for 8,192 causal tokens; packed elsewhere: 414
+            // against 424 at 64, 437 against 455 capped)
             float2 sum = dup2(0.f);
             const float2 mu = dup2(yb - u), mm = dup2(ym);
             auto ready = [&](uint64_t* bar) {  // the P stored so far may be read
@@ -670,7 +678,13 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                         const float2 y = arg(make_float2(x[k], x[k + 1]));
                         const float2 p = make_float2(ex2(y.x), ex2(y.y));
                         w[c] = Elem<T>::pack(p.x, p.y);
-                        sum = add2(sum, make_float2(Elem<T>::lo(w[c]), Elem<T>::hi(w[c])));
+                        const float2 r = make_float2(Elem<T>::lo(w[c]), Elem<T>::hi(w[c]));
+                        if constexpr (HD == 128 && !CAP) {
+                            sum.x += r.x;
+                            sum.y += r.y;
+                        } else {
+                            sum = add2(sum, r);
+                        }
                     }
                     const uint32_t at = t_lane + C::S_COL + (uint32_t)(b * BN + col + h * (N / 4));
                     if constexpr (N == 64) tmem_st16(at, w);

@@ -81,25 +81,16 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const __grid_const
     const int half = a.rope.half;
     float2* cs = cs_all + (size_t)group * half;
 
-    int64_t slot = -1;  // row of the pages (of one kv head's 16) this token goes to, in units of [nk][16]
+    int page = -1;  // the page this token goes to
     int pos = 0;
     bool live = t < a.r.n_tokens;
-    if (PAGED) {
+    if (PAGED && live) {
         // a group is whole warps of one token, so the look-up is warp-uniform
-        if (live) {
-            const int s = seq_of_token(a.r, t);
-            int t0 = 0, t1 = 0;
-            if (s < a.r.n_seqs) seq_tokens(a.r, s, t0, t1);
-            live = t >= t0 && t < t1;
-            if (live) {
-                pos = a.r.kv_len[s] - (t1 - t0) + (t - t0);
-                const int32_t* row = table_row(a.r, s);
-                if (row && pos >= 0 && pos / kPageTokens < a.r.pt_stride) {
-                    const int page = row[pos / kPageTokens];
-                    if (page >= 0 && page < a.r.n_pages) slot = (int64_t)page;
-                }
-            }
-        }
+        const TokenPlace at = place_of_token(a.r, t);
+        live = at.seq >= 0;
+        pos = at.pos;
+        if (live && at.row >= 0 && at.row < a.r.table_rows && pos >= 0 && pos / kPageTokens < a.r.pt_stride)
+            page = a.r.table[(size_t)at.row * a.r.pt_stride + pos / kPageTokens];  // (on its way until the first k head)
     }
     if (live) {
         for (int i = gt; i < half; i += a.tpt) {
@@ -134,14 +125,14 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const __grid_const
                 src = reinterpret_cast<const T*>(a.q) + (int64_t)t * a.q_stride + (int64_t)h * a.hd;
                 dst = reinterpret_cast<T*>(a.q_out) + (int64_t)t * a.q_out_stride + (int64_t)h * a.hd;
             } else {
-                if (slot < 0) continue;
+                if (page < 0 || page >= a.r.n_pages) continue;
                 const bool is_k = h < a.nq + a.nk;
                 const int hk = h - a.nq - (is_k ? 0 : a.nk);
                 src = is_k ? reinterpret_cast<const T*>(a.k) + (int64_t)t * a.k_stride
                            : reinterpret_cast<const T*>(a.v) + (int64_t)t * a.v_stride;
                 src += (int64_t)hk * a.hd;
                 dst = reinterpret_cast<T*>(is_k ? a.k_pages : a.v_pages) +
-                      ((slot * a.nk + hk) * kPageTokens + pos % kPageTokens) * (int64_t)a.hd;
+                      (((int64_t)page * a.nk + hk) * kPageTokens + pos % kPageTokens) * (int64_t)a.hd;
             }
             Unit<T, VEC> x0 = load_unit<T, VEC>(src + o0), x1 = load_unit<T, VEC>(src + o1);
             if (rot && (!PAGED || h < a.nq + a.nk)) {

@@ -220,11 +220,8 @@ ti_status ti_op_kv_append(const ti_paged_kv* kv, const ti_ragged* batch, const t
  *   z = scale q.k;  softcap > 0: z = softcap tanh(z / softcap);  slopes: z -= slopes[h] |i - j|
  * for the token at position i and key j; it sees j < kv_len[s] with
  *   j <= i or j < prefix[s],  j > i - sliding_window (when > 0),  j >= doc_start[t].
- * A token that sees nothing gets a zero row.  K and V of positions that no token
- * of the call sees never enter, whatever they hold (NaN, infinities, stale pages);
- * in ti_op_paged_prefill a V row with a NaN or an infinity may also reach tokens that
- * do not see it, where it lies within 128 positions of ones that see it and those tokens
- * share its tile. */
+ * A token that sees nothing gets a zero row.  K and V of positions that a token does
+ * not see never enter its row, whatever they hold (NaN, infinities, stale pages). */
 typedef struct {
     float scale;                /* not negative; 0: 1 / sqrt(head_dim) */
     float softcap;              /* 0: none; else scale / 1000 .. scale * 10,000 */

@@ -38,8 +38,8 @@ namespace ti {
 
 // Registers: with two streams the block is launched with 96 a thread (640 x 96 = 61,440), and the loading and
 // issuing warps hand some of theirs to the softmax warps: 128 x 64 + 512 x 104 = 61,440, or, where the cap's
-// polynomial needs them, 128 x 32 + 512 x 112 (8,192 tokens capped at head_dim 128 / 64: 437 / 523 us against 449 /
-// 556; uncapped 491 / 422 against 486 / 414).
+// polynomial needs them, 128 x 32 + 512 x 112 (8,192 tokens capped at head_dim 128 / 64: 470 / 579 us against 495 /
+// 604; uncapped 491 / 422 against 486 / 414).
 constexpr int kRegsLaunch = 96;
 constexpr int regs_other(bool cap) { return cap ? 32 : 64; }
 constexpr int regs_softmax(bool cap) { return cap ? 112 : 104; }
@@ -214,6 +214,55 @@ template <class T>
 __host__ __device__ constexpr uint32_t pre_idesc(int n, bool b_nmajor) {
     return (1u << 4) | (Elem<T>::kUmmaFmt << 7) | (Elem<T>::kUmmaFmt << 10) | (b_nmajor ? 1u << 16 : 0u) |
            ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// Half the dims of a lane's row (row_id of the CTA) once more where `odd`, one key of the CTA's [k_first, k_last) after the
+// other: sum_j p_j v_j with the row's maximum m, times inv to out, or as it is to the partial.  The row's
+// place is looked up again: kept, it would cost the softmax loop registers.  Whole warps call it.
+template <int HD, class T>
+TI_DEVICE_INLINE void odd_rows(const PreArgs& a, int row_id, int half, int k_first, int k_last, bool odd, float m, float inv) {
+    const RowTile rt = find_rows<PreCfg<HD>::ROWS>(a, blockIdx.x / a.p.n_kv);
+    if (!odd) return;
+    const int hk = blockIdx.x % a.p.n_kv, r = rt.row0 + row_id;
+    const int token = rt.t0 + r / a.group, head = hk * a.group + r % a.group, pos = rt.kv_len - (rt.t1 - token);
+    const int32_t* table = a.p.r.table + (size_t)rt.row * a.p.r.pt_stride;  // (a row that saw keys has one)
+    int lo, hi;
+    key_range(a.p.f, rt.seq, token, pos, min(rt.kv_len, a.p.r.pt_stride * kPageTokens), lo, hi);
+    lo = max(lo, k_first);
+    hi = min(hi, k_last);
+    const T* q = reinterpret_cast<const T*>(a.p.q) + (int64_t)token * a.p.q_stride + (int64_t)head * HD;
+    T* dst = reinterpret_cast<T*>(a.p.out) + (int64_t)token * a.p.out_stride + (int64_t)head * HD;
+    float* part = a.part_o + (((int64_t)blockIdx.z * a.p.r.n_tokens + token) * a.p.n_heads + head) * HD;
+    const float slope = a.p.f.slopes ? a.p.f.slopes[head] : 0.f;
+    constexpr int N = 16;  // dims a pass
+#pragma unroll 1
+    for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += N) {
+        float acc[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] = 0.f;
+#pragma unroll 1
+        for (int j = lo; j < hi; ++j) {
+            const int id = table[j / kPageTokens];
+            if (id < 0 || id >= a.p.r.n_pages) continue;  // values of zero
+            const int64_t at = (((int64_t)id * a.p.n_kv + hk) * kPageTokens + j % kPageTokens) * HD;
+            const T* k = reinterpret_cast<const T*>(a.p.k_pages) + at;
+            const T* v = reinterpret_cast<const T*>(a.p.v_pages) + at + d;
+            float z = 0.f;
+#pragma unroll 4
+            for (int e = 0; e < HD; ++e) z = fmaf(Elem<T>::to_f(q[e]), Elem<T>::to_f(k[e]), z);
+            z *= a.p.f.scale;
+            if (a.p.f.cap > 0.f) z = a.p.f.cap * tanhf(z / a.p.f.cap);
+            z -= slope * fabsf((float)(pos - j));
+            const float p = Elem<T>::to_f(Elem<T>::from_f(ex2(fmaf(z, kLog2E, -m))));
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] = fmaf(p, Elem<T>::to_f(v[i]), acc[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (a.splits > 1) part[d + i] = acc[i];
+            else dst[d + i] = Elem<T>::from_f(acc[i] * inv);
+        }
+    }
 }
 
 template <int HD, class T, bool CAP, bool BIAS>
@@ -657,8 +706,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 if (grow) m = mx;
             }
             const float u = m == -INFINITY ? 0.f : m;
-            // (scalar sums uncapped at head_dim 128: 474 against 486 us for 8,192 causal tokens; packed elsewhere: 414
-            // against 424 at 64, 437 against 455 capped)
+            // (scalar sums at head_dim 128: 474 against 486 us for 8,192 causal tokens, capped 470 against 493; packed
+            // elsewhere: 414 against 424 at 64)
             float2 sum = dup2(0.f);
             const float2 mu = dup2(yb - u), mm = dup2(ym);
             auto ready = [&](uint64_t* bar) {  // the P stored so far may be read
@@ -679,7 +728,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                         const float2 p = make_float2(ex2(y.x), ex2(y.y));
                         w[c] = Elem<T>::pack(p.x, p.y);
                         const float2 r = make_float2(Elem<T>::lo(w[c]), Elem<T>::hi(w[c]));
-                        if constexpr (HD == 128 && !CAP) {
+                        if constexpr (HD == 128) {
                             sum.x += r.x;
                             sum.y += r.y;
                         } else {
@@ -706,6 +755,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             good = __all_sync(0xffffffffu, pipe_wait(&o_full[q], 0, stop));
             tc_fence_after();
         }
+        float odd = 0.f;  // NaN once one of the thread's outputs is a NaN or an infinity
         if (a.splits > 1) {
             const int64_t row = ((int64_t)blockIdx.z * a.p.r.n_tokens + token) * a.p.n_heads + head;
             if (mine && half == 0) reinterpret_cast<float2*>(a.part_ml)[row] = nt > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
@@ -713,6 +763,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                     float o[32];
                     tmem_ld32(t_lane + C::O_COL + (uint32_t)(q * HD + c), o);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) odd = fmaf(o[k], 0.f, odd);
                     if (mine)
 #pragma unroll
                         for (int k = 0; k < 32; k += 4)
@@ -727,7 +779,11 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                 float o[32];
                 uint32_t w[16];
-                if (nt > 0) tmem_ld32(t_lane + C::O_COL + (uint32_t)(q * HD + c), o);
+                if (nt > 0) {
+                    tmem_ld32(t_lane + C::O_COL + (uint32_t)(q * HD + c), o);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) odd = fmaf(o[k], 0.f, odd);
+                }
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
                     w[k] = nt > 0 && l != 0.f ? Elem<T>::pack(o[2 * k] * inv, o[2 * k + 1] * inv) : 0u;
@@ -745,6 +801,12 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 }
             }
         }
+        // A NaN or an infinity in V meets rows of its tile that do not see it with a probability of zero, and
+        // zero times it is NaN.  A thread with such outputs makes them once more, from the keys its row sees alone.
+        // (Taking such values out of V before the MMAs read it costs each tile with a partly seen key some 3,000
+        // cycles: 23 -> 37 us for short prompts.)
+        const bool again = mine && odd != 0.f && l == l && l != 0.f;
+        if (__any_sync(0xffffffffu, again)) odd_rows<HD, T>(a, row_id, half, j0 * BN, j1 * BN, again, m, 1.f / l);
     }
     tc_fence_before();
     __syncthreads();

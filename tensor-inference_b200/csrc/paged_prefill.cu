@@ -758,7 +758,9 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         float odd = 0.f;  // NaN once one of the thread's outputs is a NaN or an infinity
         if (a.splits > 1) {
             const int64_t row = ((int64_t)blockIdx.z * a.p.r.n_tokens + token) * a.p.n_heads + head;
-            if (mine && half == 0) reinterpret_cast<float2*>(a.part_ml)[row] = nt > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+            // (a row that saw none of these keys has no part in the join, whatever zero times V came to)
+            if (mine && half == 0)
+                reinterpret_cast<float2*>(a.part_ml)[row] = nt > 0 && l != 0.f ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
             if (nt > 0 && good) {
                 for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                     float o[32];

@@ -445,38 +445,38 @@ def test_nan_outside_the_mask_does_not_enter(entry):
     assert torch.equal(out, clean)
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dtype, cap", [("bf16", 0.0), ("bf16", 20.0), ("f16", 0.0), ("f16", 20.0)])
 @pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("window, max_len", [(90, 200), (0, 200), (0, 4096)])  # the last: keys divided over CTAs
 @pytest.mark.parametrize("odd", [[61], [3, 61, 62, 130], list(range(20, 120))])
-def test_nan_and_infinities_in_v_reach_the_rows_that_see_them(odd, hd, dtype):
+def test_nan_and_infinities_in_v_reach_the_rows_that_see_them(odd, window, max_len, hd, dtype, cap):
     # rows before the key, or whose window has passed it, share its tiles and stay finite; the others get a NaN
     # or an infinity of its sign in that dimension alone
-    heads, window = 4, 90
+    heads = 4
     c = Cache([(150, 200)], 2, hd, dtype, seed=13)
+    c.max_len = max_len
     q = queries(c, heads)
-    clean, ref, tol = run_attention(c, q, heads, "prefill", window=window)
+    clean, ref, tol = run_attention(c, q, heads, "prefill", window=window, cap=cap)
     within(clean, ref, tol)
-    for splits in (False, True):
-        d = c.dev()
-        d["batch"].max_len = 4096 if splits else 16  # (how the keys are divided over CTAs)
-        values = [float("nan"), float("inf"), -float("inf")]
-        want = np.zeros((150, heads, hd))
-        for n, j in enumerate(odd):
-            page, dim, h = int(c.table[c.rows[0], j // 16]), (7 * j) % hd, j % 2
-            d["v"][page, h, j % 16, dim] = values[n % 3]
-            i = np.arange(50, 200)
-            rows = (i >= j) & (i - j < window)
-            with np.errstate(invalid="ignore"):
-                want[rows, 2 * h:2 * h + 2, dim] += values[n % 3]
-        out, _, _ = run_attention(c, q, heads, "prefill", window=window, d=d)
-        got = out.cpu().double().numpy()
-        fine = want == 0
-        assert np.isfinite(got[fine]).all()
-        # the odd values are single dimensions of V: every other output keeps its value
-        assert (np.abs(got - ref)[fine] <= tol[fine]).all()
-        np.testing.assert_array_equal(np.isnan(got[~fine]), np.isnan(want[~fine]))
-        inf = ~fine & np.isinf(want)
-        np.testing.assert_array_equal(got[inf], want[inf])
+    d = c.dev()
+    values = [float("nan"), float("inf"), -float("inf")]
+    want = np.zeros((150, heads, hd))
+    for n, j in enumerate(odd):
+        page, dim, h = int(c.table[c.rows[0], j // 16]), (7 * j) % hd, j % 2
+        d["v"][page, h, j % 16, dim] = values[n % 3]
+        i = np.arange(50, 200)
+        rows = (i >= j) & ((i - j < window) | (window == 0))
+        with np.errstate(invalid="ignore"):
+            want[rows, 2 * h:2 * h + 2, dim] += values[n % 3]
+    out, _, _ = run_attention(c, q, heads, "prefill", window=window, cap=cap, d=d)
+    got = out.cpu().double().numpy()
+    fine = want == 0
+    assert np.isfinite(got[fine]).all()
+    # the odd values are single dimensions of V: every other output keeps its value
+    assert (np.abs(got - ref)[fine] <= tol[fine]).all()
+    np.testing.assert_array_equal(np.isnan(got[~fine]), np.isnan(want[~fine]))
+    inf = ~fine & np.isinf(want)
+    np.testing.assert_array_equal(got[inf], want[inf])
 
 
 def test_lowest_values_in_keys_are_ordinary_scores():

@@ -221,7 +221,9 @@ ti_status ti_op_kv_append(const ti_paged_kv* kv, const ti_ragged* batch, const t
  * for the token at position i and key j; it sees j < kv_len[s] with
  *   j <= i or j < prefix[s],  j > i - sliding_window (when > 0),  j >= doc_start[t].
  * A token that sees nothing gets a zero row.  K and V of positions that a token does
- * not see never enter its row, whatever they hold (NaN, infinities, stale pages). */
+ * not see never enter its row, whatever they hold (NaN, infinities, stale pages).
+ * A NaN or an infinity in V of a position that it does see makes that dimension of its
+ * row a NaN or that infinity, however small the position's weight. */
 typedef struct {
     float scale;                /* not negative; 0: 1 / sqrt(head_dim) */
     float softcap;              /* 0: none; else scale / 1000 .. scale * 10,000 */

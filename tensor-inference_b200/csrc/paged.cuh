@@ -27,6 +27,7 @@ struct Elem;
 template <>
 struct Elem<__nv_bfloat16> {
     static constexpr uint32_t kUmmaFmt = 1;  // tcgen05 kind::f16 operand format
+    static constexpr uint32_t kExp = 0x7f80u;  // the exponent's bits: all set in an infinity or a NaN
     static TI_DEVICE_INLINE float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
     static TI_DEVICE_INLINE __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
     static TI_DEVICE_INLINE float lo(uint32_t u) { return __uint_as_float(u << 16); }
@@ -40,6 +41,7 @@ struct Elem<__nv_bfloat16> {
 template <>
 struct Elem<__half> {
     static constexpr uint32_t kUmmaFmt = 0;
+    static constexpr uint32_t kExp = 0x7c00u;
     static TI_DEVICE_INLINE float to_f(__half v) { return __half2float(v); }
     static TI_DEVICE_INLINE __half from_f(float v) { return __float2half_rn(v); }
     static TI_DEVICE_INLINE float lo(uint32_t u) { return __half2float(__ushort_as_half((unsigned short)(u & 0xffffu))); }
@@ -55,6 +57,27 @@ struct Elem<float> {
     static TI_DEVICE_INLINE float to_f(float v) { return v; }
     static TI_DEVICE_INLINE float from_f(float v) { return v; }
 };
+
+// ------------------------------------------------------------------ infinities and NaN among values
+// two bits for each of eight 16-bit values: 1 +infinity, 2 -infinity, 3 NaN, 0 finite (or-ed together: what a
+// weighted sum of them with weights above zero comes to)
+template <class T>
+TI_DEVICE_INLINE uint32_t odd_kinds(const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    constexpr uint32_t E = Elem<T>::kExp;
+    uint32_t kinds = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t e = w[i / 2] >> (i % 2 * 16) & 0xffffu;
+        if ((e & E) == E) kinds |= ((e & 0x7fffu) != E ? 3u : e >> 15 ? 2u : 1u) << (2 * i);
+    }
+    return kinds;
+}
+TI_DEVICE_INLINE float odd_value(uint32_t kind) {
+    return kind == 1 ? INFINITY : kind == 2 ? -INFINITY : __int_as_float(0x7fffffff);
+}
+// a partial output times its weight: an infinity counts even where its weight has come to zero
+TI_DEVICE_INLINE float join_add(float o, float v, float f) { return fabsf(v) == INFINITY ? o + v : fmaf(v, f, o); }
 
 // ------------------------------------------------------------------ ragged batch
 struct RaggedDev {

@@ -192,6 +192,17 @@ TI_DEVICE_INLINE uint32_t swz(int C, int row, int d) {
     return (uint32_t)((d >> 6) * C + row) * 128u + (uint32_t)((((d & 63) >> 3) ^ (row & 7)) << 4) + (uint32_t)((d & 7) << 1);
 }
 
+// whether `v` holds in one of the consumer warps; a barrier among them
+TI_DEVICE_INLINE bool consumers_or(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.or.pred q, 1, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+        : "=r"(r)
+        : "r"((uint32_t)v), "n"(kDecWarps * 32)
+        : "memory");
+    return r != 0;
+}
+
 // G16: the segment has more than 8 heads
 template <int HD, class T, bool G16>
 __global__ void __launch_bounds__(kDecThreads, 1)
@@ -512,6 +523,9 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         named_bar(1, kDecWarps * 32);
         // (the next write to this area comes after the next segment's barrier for q)
         const bool whole = p0 == 0 && p1 == x.npg;
+        T* out = reinterpret_cast<T*>(a.p.out) + (int64_t)s * a.p.out_stride + (int64_t)h0 * HD;
+        float* part = a.part_o + ((int64_t)blockIdx.x * 2 + (seg_no ? 1 : 0)) * a.rows * HD;
+        bool odd = false;  // one of the thread's outputs is a NaN that the scores do not explain
         for (int e = tid * 4; e < G * HD; e += kDecWarps * 32 * 4) {
             const int r = e / HD, d = e % HD, dpart = d / DW;
             float2 st[NG];
@@ -534,9 +548,12 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                 v.z = fmaf(y.z, f, v.z);
                 v.w = fmaf(y.w, f, v.w);
             }
+            if (l == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);  // every score -inf: no weight, whatever V holds
+            const float any = v.x + v.y + v.z + v.w;
+            odd |= any != any && l == l;
             if (whole) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                T* dst = reinterpret_cast<T*>(a.p.out) + (int64_t)s * a.p.out_stride + (int64_t)(h0 + r) * HD + d;
+                T* dst = out + e;
                 if (a.out_vec) {
                     *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(v.x * inv, v.y * inv), Elem<T>::pack(v.z * inv, v.w * inv));
                 } else {
@@ -547,8 +564,40 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                 }
             } else {
                 const int64_t row = ((int64_t)blockIdx.x * 2 + (seg_no ? 1 : 0)) * a.rows + r;
-                __stcg(reinterpret_cast<float4*>(a.part_o + row * HD + d), v);
+                __stcg(reinterpret_cast<float4*>(part + e), v);
                 if (d == 0) __stcg(reinterpret_cast<float2*>(a.part_ml) + row, make_float2(M, l));
+            }
+        }
+        if (consumers_or(odd)) {
+            // An infinity in V meets the low term of a probability, which may be zero or negative, and becomes a NaN.  The
+            // stretch's V is read once more: a dimension with a NaN, or infinities of both signs, is a NaN, one with
+            // infinities of one sign that infinity, whatever their weights.
+            uint32_t* kinds = reinterpret_cast<uint32_t*>(red);  // [HD / 8]: two bits a dimension
+            constexpr int CH = HD / 8, KR = kDecWarps * 32 / CH;
+            if (tid < CH) kinds[tid] = 0;
+            named_bar(1, kDecWarps * 32);
+            const int ja = max(x.lo, (x.pg0 + p0) * kPageTokens), jb = min(x.hi, (x.pg0 + p1) * kPageTokens);
+            uint32_t seen = 0;
+#pragma unroll 4
+            for (int j = ja + tid / CH; j < jb; j += KR) {
+                const int id = x.row[j / kPageTokens];
+                if (id < 0 || id >= a.p.r.n_pages) continue;
+                const int64_t at = (((int64_t)id * a.p.n_kv + hk) * kPageTokens + j % kPageTokens) * HD + tid % CH * 8;
+                seen |= odd_kinds<T>(*reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.p.v_pages) + at));
+            }
+            if (seen) atomicOr(&kinds[tid % CH], seen);
+            named_bar(1, kDecWarps * 32);
+            for (int e = tid * 4; e < G * HD; e += kDecWarps * 32 * 4) {
+                const int r = e / HD, d = e % HD, dpart = d / DW;
+                float l = 0.f;
+                for (int w = 0; w < NG; ++w) l += ml[(w * DPARTS + dpart) * 32 + r * 2 + 1];
+                if (!(l > 0.f)) continue;  // (a NaN of the scores stays)
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t kind = kinds[d / 8] >> ((d % 8 + k) * 2) & 3u;
+                    if (kind == 0) continue;
+                    if (whole) out[e + k] = Elem<T>::from_f(odd_value(kind));
+                    else __stcg(part + e + k, odd_value(kind));
+                }
             }
         }
         it += n_st;
@@ -607,10 +656,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_consta
         for (int c = 0; c < nc; ++c) {
             const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + row_of(c0 + c, r) * HD + d));
             const float f = w[c * kDecRows + r];
-            o.x = fmaf(v.x, f, o.x);
-            o.y = fmaf(v.y, f, o.y);
-            o.z = fmaf(v.z, f, o.z);
-            o.w = fmaf(v.w, f, o.w);
+            o.x = join_add(o.x, v.x, f);
+            o.y = join_add(o.y, v.y, f);
+            o.z = join_add(o.z, v.z, f);
+            o.w = join_add(o.w, v.w, f);
         }
         out[e] = Elem<T>::from_f(o.x * inv[r]);
         out[e + 1] = Elem<T>::from_f(o.y * inv[r]);

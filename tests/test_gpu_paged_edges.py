@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import ti_b200 as ti
-from paged_ref import DT, Cache
+from paged_ref import DT, Cache, attend
 from test_gpu_paged_ops import queries, run_attention, stream, within
 
 pytestmark = pytest.mark.gpu
@@ -28,6 +28,47 @@ def same_odd_values(got, want, ref, tol):
     np.testing.assert_array_equal(np.isnan(got[~fine]), np.isnan(want[~fine]))
     inf = np.isinf(want)
     np.testing.assert_array_equal(got[inf], want[inf])
+
+
+def forms(c, heads, cap=0.0, bias=False, window=0, prefix=False, docs=0, scale=0.0):
+    """arguments of `attend` for masks that differ from sequence to sequence and token to token"""
+    slopes = (2.0 ** (-6.0 * (np.arange(heads) + 1) / heads)).astype(np.float32) if bias else None
+    pre = np.array([(37 * (s + 3)) % (c.max_len + 9) for s in range(len(c.seqs))], np.int32) if prefix else None
+    doc = None
+    if docs:
+        doc = np.zeros(c.tokens, np.int32)
+        for s, (new, n) in enumerate(c.seqs):
+            i = np.arange(n - new, n)
+            doc[c.starts[s]:c.starts[s] + new] = i - i % docs
+    return dict(cap=cap, slopes=slopes, window=window, prefix=pre, doc=doc, scale=scale)
+
+
+def launch(c, d, q, heads, entry, form, out=None):
+    dev = {k: torch.from_numpy(form[k]).cuda() for k in ("slopes", "prefix", "doc") if form[k] is not None}
+    at = {k: v.data_ptr() for k, v in dev.items()}
+    f = ti.AttnForm(scale=form["scale"], softcap=form["cap"], slopes=at.get("slopes"), sliding_window=form["window"],
+                    prefix=at.get("prefix"), doc_start=at.get("doc"))
+    dq = q.cuda()
+    if out is None:
+        out = torch.full((c.tokens, heads, c.hd), 3.0, dtype=DT[c.dtype], device="cuda")
+    ti.check(getattr(ti.lib(), f"ti_op_paged_{entry}")(C.byref(d["kv"]), C.byref(d["batch"]), C.byref(f), dq.data_ptr(),
+                                                       heads * c.hd, heads, out.data_ptr(), heads * c.hd, stream()))
+    torch.cuda.synchronize()
+    return out
+
+
+def sees(c, s, j, form):
+    """which new tokens of sequence s see position j"""
+    new, n = c.seqs[s]
+    i = np.arange(n - new, n)
+    ok = i >= j
+    if form["prefix"] is not None:
+        ok = ok | (j < form["prefix"][s])
+    if form["window"]:
+        ok = ok & (j > i - form["window"])
+    if form["doc"] is not None:
+        ok = ok & (j >= form["doc"][c.starts[s]:c.starts[s] + new])
+    return ok
 
 
 # ------------------------------------------------------------------ infinities and NaN in V
@@ -91,3 +132,20 @@ def test_decode_infinity_counts_however_small_its_weight(length, dtype):
     want[..., 3], want[..., 40], want[..., 5] = np.inf, -np.inf, np.nan
     out, _, _ = run_attention(c, q, 2, "decode", d=d)
     same_odd_values(out, want, ref, tol)
+
+
+@pytest.mark.parametrize("hd, dtype", [(64, "bf16"), (128, "f16"), (256, "bf16")])
+def test_prefill_join_keeps_the_odd_values_of_a_share_without_weight(hd, dtype):
+    # keys divided over CTAs, and a distance bias that leaves the first share no weight in fp32: its NaN still counts
+    heads = 2
+    c = Cache([(20, 1500)], 1, hd, dtype, seed=37)
+    f = forms(c, heads)
+    f["slopes"] = np.array([0.5, 0.25], np.float32)
+    q = queries(c, heads)
+    ref, tol = attend(c, q, heads, **f)
+    d = c.dev()
+    within(launch(c, d, q, heads, "prefill", f), ref, tol)
+    put(c, d["v"], 0, 3, 0, 17, float("nan"))
+    want = np.zeros((20, heads, hd))
+    want[..., 17] = np.nan
+    same_odd_values(launch(c, d, q, heads, "prefill", f), want, ref, tol)

@@ -73,11 +73,59 @@ TI_DEVICE_INLINE uint32_t odd_kinds(const uint4& v) {
     }
     return kinds;
 }
+// takes the infinities and NaN out of v (zeros for them)
+template <class T>
+TI_DEVICE_INLINE void finite_only(uint4& v) {
+    constexpr uint32_t E = Elem<T>::kExp;
+    auto keep = [](uint32_t w) {
+        return w & (((w & E) == E ? 0u : 0xffffu) | ((w >> 16 & E) == E ? 0u : 0xffff0000u));
+    };
+    v = make_uint4(keep(v.x), keep(v.y), keep(v.z), keep(v.w));
+}
 TI_DEVICE_INLINE float odd_value(uint32_t kind) {
     return kind == 1 ? INFINITY : kind == 2 ? -INFINITY : __int_as_float(0x7fffffff);
 }
 // a partial output times its weight: an infinity counts even where its weight has come to zero
 TI_DEVICE_INLINE float join_add(float o, float v, float f) { return fabsf(v) == INFINITY ? o + v : fmaf(v, f, o); }
+
+// ------------------------------------------------------------------ warp-level products
+TI_DEVICE_INLINE void ldsm4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+                 : "r"(addr));
+}
+TI_DEVICE_INLINE void ldsm4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+                 : "r"(addr));
+}
+template <class T>
+TI_DEVICE_INLINE void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
+template <>
+TI_DEVICE_INLINE void mma16<__nv_bfloat16>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+TI_DEVICE_INLINE void mma16<__half>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// byte offset of (row, d) in a [HD/64][C][64] tile of 16-bit elements with 128-byte swizzled rows
+TI_DEVICE_INLINE uint32_t swz(int C, int row, int d) {
+    return (uint32_t)((d >> 6) * C + row) * 128u + (uint32_t)((((d & 63) >> 3) ^ (row & 7)) << 4) + (uint32_t)((d & 7) << 1);
+}
+
+// two probabilities as 16-bit pairs hi + lo
+template <class T>
+TI_DEVICE_INLINE void split_p(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+    hi = Elem<T>::pack(p0, p1);
+    lo = Elem<T>::pack(p0 - Elem<T>::lo(hi), p1 - Elem<T>::hi(hi));
+}
 
 // ------------------------------------------------------------------ ragged batch
 struct RaggedDev {

@@ -161,37 +161,6 @@ TI_DEVICE_INLINE Line find_line(const DecArgs& a, int cta, int ctas, int want, i
     return L;
 }
 
-TI_DEVICE_INLINE void ldsm4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-                 : "r"(addr));
-}
-TI_DEVICE_INLINE void ldsm4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-                 : "r"(addr));
-}
-template <class T>
-TI_DEVICE_INLINE void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
-template <>
-TI_DEVICE_INLINE void mma16<__nv_bfloat16>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-TI_DEVICE_INLINE void mma16<__half>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// byte offset of (row, d) in a [HD/64][C][64] tile of 16-bit elements with 128-byte swizzled rows
-TI_DEVICE_INLINE uint32_t swz(int C, int row, int d) {
-    return (uint32_t)((d >> 6) * C + row) * 128u + (uint32_t)((((d & 63) >> 3) ^ (row & 7)) << 4) + (uint32_t)((d & 7) << 1);
-}
-
 // whether `v` holds in one of the consumer warps; a barrier among them
 TI_DEVICE_INLINE bool consumers_or(bool v) {
     uint32_t r;
@@ -476,15 +445,11 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                 }
                 // ---- P.V, P = hi + lo in 16 bits: what the two drop is under 2^-16 of p (bf16) or 2^-22 (f16)
                 uint32_t ph[4], pl[4];
-                auto split = [](float p0_, float p1_, uint32_t& hi, uint32_t& lo) {
-                    hi = Elem<T>::pack(p0_, p1_);
-                    lo = Elem<T>::pack(p0_ - Elem<T>::lo(hi), p1_ - Elem<T>::hi(hi));
-                };
-                split(c[0][0], c[0][1], ph[0], pl[0]);
-                split(c[1][0], c[1][1], ph[2], pl[2]);
+                split_p<T>(c[0][0], c[0][1], ph[0], pl[0]);
+                split_p<T>(c[1][0], c[1][1], ph[2], pl[2]);
                 if constexpr (G16) {
-                    split(c[0][2], c[0][3], ph[1], pl[1]);
-                    split(c[1][2], c[1][3], ph[3], pl[3]);
+                    split_p<T>(c[0][2], c[0][3], ph[1], pl[1]);
+                    split_p<T>(c[1][2], c[1][3], ph[3], pl[3]);
                 } else {
                     ph[1] = pl[1] = ph[3] = pl[3] = 0u;
                 }

@@ -27,6 +27,9 @@
 // Few rows over a long cache: the key tiles of a row tile are divided over gridDim.z CTAs,
 // whose partial (max, sum, output) rows k_prefill_join adds in order.
 //
+// A NaN or an infinity in V meets the rows of its tile that do not see it with a probability of zero, and zero
+// times it is NaN.  A CTA with an output that is not finite looks at its keys once more when it is done (settle_odd).
+//
 // Every wait is bounded; one that gives up stops all roles, the MMAs issued are waited for, and TMEM is freed.
 #include <algorithm>
 #include <atomic>
@@ -216,51 +219,281 @@ __host__ __device__ constexpr uint32_t pre_idesc(int n, bool b_nmajor) {
            ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-// Half the dims of a lane's row (row_id of the CTA) once more where `odd`, one key of the CTA's [k_first, k_last) after the
-// other: sum_j p_j v_j with the row's maximum m, times inv to out, or as it is to the partial.  The row's
-// place is looked up again: kept, it would cost the softmax loop registers.  Whole warps call it.
+// A softmax thread's row: token, head, position and the keys [lo, hi) that it sees.  (Softmax warps
+// 8 q + 4 half + quarter: the row of lane l is 128 q + 32 quarter + l.)
+struct Row {
+    int id, token, head, pos, lo, hi;
+    bool mine;  // there is such a row
+};
+template <int HD>
+TI_DEVICE_INLINE Row row_of(const PreArgs& a, const RowTile& rt, int hk, int id, int n_keys) {
+    Row x{id, 0, 0, 0, 0, 0, false};
+    const int r = rt.row0 + id;
+    x.mine = id < PreCfg<HD>::ROWS && r < (rt.t1 - rt.t0) * a.group;
+    if (x.mine) {
+        x.token = rt.t0 + r / a.group;
+        x.head = hk * a.group + r % a.group;
+        x.pos = rt.kv_len - (rt.t1 - x.token);
+        key_range(a.p.f, rt.seq, x.token, x.pos, n_keys, x.lo, x.hi);
+    }
+    return x;
+}
+// key tiles [j0, j1) of this CTA: its share of those with keys [key_lo, key_hi)
+template <int BN>
+TI_DEVICE_INLINE void key_tiles(const PreArgs& a, int key_lo, int key_hi, int& j0, int& j1) {
+    j0 = key_hi > key_lo ? key_lo / BN : 0;
+    j1 = key_hi > key_lo ? (key_hi + BN - 1) / BN : 0;
+    if (a.splits > 1) {
+        const int per = (j1 - j0 + a.splits - 1) / a.splits;
+        j0 = min(j1, j0 + (int)blockIdx.z * per);
+        j1 = min(j1, j0 + per);
+    }
+}
+// whether `v` holds in one of the softmax threads; a barrier among them
+template <int THREADS>
+TI_DEVICE_INLINE bool softmax_or(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.or.pred q, 11, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+        : "=r"(r)
+        : "r"((uint32_t)v), "n"(THREADS)
+        : "memory");
+    return r != 0;
+}
+
+// After a pass that left outputs which are not finite.  `settle`: the thread's row saw keys, and its scores are no NaN.
+// First the CTA reads the V of its keys once more and finds which rows see infinities and NaN in which dimensions: an
+// infinity of one sign stays one, everything else is a NaN, whatever the weights.  A NaN that this does
+// not explain came from values that its row does not see.  Those outputs are computed again, 64 dims at a
+// time, with such values taken out of V: 16 rows a warp on mma.sync, keys in tiles through shared
+// memory, P as two 16-bit terms.  It looks the rows up again, so that the kernel's loop keeps no more than it needs: it
+// costs 8,192 causal tokens 0 to 2% of their time (as a called function 2 to 6%).  (Taking the values out of V before the MMAs read it costs each tile with a partly seen key some
+// 3,000 cycles: 23 -> 37 us for short prompts.)
 template <int HD, class T>
-TI_DEVICE_INLINE void odd_rows(const PreArgs& a, int row_id, int half, int k_first, int k_last, bool odd, float m, float inv) {
-    const RowTile rt = find_rows<PreCfg<HD>::ROWS>(a, blockIdx.x / a.p.n_kv);
-    if (!odd) return;
-    const int hk = blockIdx.x % a.p.n_kv, r = rt.row0 + row_id;
-    const int token = rt.t0 + r / a.group, head = hk * a.group + r % a.group, pos = rt.kv_len - (rt.t1 - token);
-    const int32_t* table = a.p.r.table + (size_t)rt.row * a.p.r.pt_stride;  // (a row that saw keys has one)
-    int lo, hi;
-    key_range(a.p.f, rt.seq, token, pos, min(rt.kv_len, a.p.r.pt_stride * kPageTokens), lo, hi);
-    lo = max(lo, k_first);
-    hi = min(hi, k_last);
-    const T* q = reinterpret_cast<const T*>(a.p.q) + (int64_t)token * a.p.q_stride + (int64_t)head * HD;
-    T* dst = reinterpret_cast<T*>(a.p.out) + (int64_t)token * a.p.out_stride + (int64_t)head * HD;
-    float* part = a.part_o + (((int64_t)blockIdx.z * a.p.r.n_tokens + token) * a.p.n_heads + head) * HD;
-    const float slope = a.p.f.slopes ? a.p.f.slopes[head] : 0.f;
-    constexpr int N = 16;  // dims a pass
-#pragma unroll 1
-    for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); d += N) {
-        float acc[N];
+TI_DEVICE_INLINE void settle_odd(const PreArgs& a, uint8_t* smem, uint32_t tmem, bool settle) {
+    using C = PreCfg<HD>;
+    constexpr PreSmem L = pre_smem<HD>();
+    constexpr int BN = C::BN, W = BN / 32, CH = HD / 8, TH = C::SW * 32, HW = HD / 64, KW = HD / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int hk = blockIdx.x % a.p.n_kv;
+    const RowTile rt = find_rows<C::ROWS>(a, blockIdx.x / a.p.n_kv);
+    const int32_t* table = a.p.r.table + (size_t)rt.row * a.p.r.pt_stride;  // (rows that saw keys: there is one)
+    const int n_keys = min(rt.kv_len, a.p.r.pt_stride * kPageTokens);
+    int key_lo = reinterpret_cast<int*>(smem + L.misc)[2], key_hi = reinterpret_cast<int*>(smem + L.misc)[3], j0, j1;
+    key_tiles<BN>(a, key_lo, key_hi, j0, j1);
+    key_lo = max(key_lo, j0 * BN);
+    key_hi = min(key_hi, j1 * BN);
+    auto value_at = [&](const void* pages, int j, int d) {  // eight dims of key j, zeros of a page that does not exist
+        const int id = table[j / kPageTokens];
+        if (id < 0 || id >= a.p.r.n_pages) return make_uint4(0, 0, 0, 0);
+        return *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(pages) +
+                                               (((int64_t)id * a.p.n_kv + hk) * kPageTokens + j % kPageTokens) * HD + d);
+    };
+    // (the K and V stages are free: every copy has landed and every MMA is done)
+    uint32_t* planes = reinterpret_cast<uint32_t*>(smem + L.k);  // odd values of a tile: [+inf or NaN, -inf or NaN][HD][BN] bits
+    uint32_t* open = planes + 2 * HD * W;                        // outputs to compute again: [HD/32][rows]
+    bool redo = false;
+    {
+        const int half = (warp >> 2) & 1;
+        const Row x = row_of<HD>(a, rt, hk, (warp >> 3) * 128 + (warp & 3) * 32 + lane, n_keys);
+        const int lo = settle ? x.lo : 0, hi = settle ? x.hi : 0;
+        uint32_t seen[2][HW];
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] = 0.f;
-#pragma unroll 1
-        for (int j = lo; j < hi; ++j) {
-            const int id = table[j / kPageTokens];
-            if (id < 0 || id >= a.p.r.n_pages) continue;  // values of zero
-            const int64_t at = (((int64_t)id * a.p.n_kv + hk) * kPageTokens + j % kPageTokens) * HD;
-            const T* k = reinterpret_cast<const T*>(a.p.k_pages) + at;
-            const T* v = reinterpret_cast<const T*>(a.p.v_pages) + at + d;
-            float z = 0.f;
+        for (int w = 0; w < HW; ++w) seen[0][w] = seen[1][w] = 0;
+        auto clear = [&] {
+            for (int i = tid; i < 2 * HD * W; i += TH) planes[i] = 0;
+            softmax_or<TH>(false);
+        };
+        clear();
+        for (int k0 = j0 * BN; k0 < key_hi; k0 += BN) {
+            bool found = false;
+#pragma unroll 2
+            for (int c = tid; c < BN * CH; c += TH) {
+                const int r = c / CH, d = c % CH * 8;
+                if (k0 + r < key_lo || k0 + r >= key_hi) continue;
+                const uint32_t odd = odd_kinds<T>(value_at(a.p.v_pages, k0 + r, d));
+                if (odd == 0) continue;
+                found = true;
+                for (int e = 0; e < 16; ++e)
+                    if (odd >> e & 1u) atomicOr(&planes[((e & 1) * HD + d + e / 2) * W + r / 32], 1u << (r % 32));
+            }
+            if (!softmax_or<TH>(found)) continue;
+            uint32_t mask[W];  // the tile's keys that the row sees
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const int b0 = min(max(lo - k0 - 32 * w, 0), 32), b1 = min(max(hi - k0 - 32 * w, 0), 32);
+                mask[w] = (b1 == 32 ? ~0u : (1u << b1) - 1u) & ~(b0 == 32 ? ~0u : (1u << b0) - 1u);
+            }
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int w = 0; w < HW; ++w)
 #pragma unroll 4
-            for (int e = 0; e < HD; ++e) z = fmaf(Elem<T>::to_f(q[e]), Elem<T>::to_f(k[e]), z);
-            z *= a.p.f.scale;
-            if (a.p.f.cap > 0.f) z = a.p.f.cap * tanhf(z / a.p.f.cap);
-            z -= slope * fabsf((float)(pos - j));
-            const float p = Elem<T>::to_f(Elem<T>::from_f(ex2(fmaf(z, kLog2E, -m))));
+                    for (int b = 0; b < 32; ++b) {
+                        const uint32_t* plane = planes + (p * HD + half * (HD / 2) + w * 32 + b) * W;
+                        uint32_t any = 0;
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] = fmaf(p, Elem<T>::to_f(v[i]), acc[i]);
+                        for (int k = 0; k < W; ++k) any |= plane[k] & mask[k];
+                        seen[p][w] |= (uint32_t)(any != 0) << b;
+                    }
+            softmax_or<TH>(false);
+            clear();
+        }
+        __syncwarp();
+        T* dst = reinterpret_cast<T*>(a.p.out) + (int64_t)x.token * a.p.out_stride + (int64_t)x.head * HD;
+        float* part = a.part_o + (((int64_t)blockIdx.z * a.p.r.n_tokens + x.token) * a.p.n_heads + x.head) * HD;
+#pragma unroll
+        for (int w = 0; w < HW; ++w) {
+            float o[32];
+            tmem_ld32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + C::O_COL +
+                          (uint32_t)((warp >> 3) * HD + half * (HD / 2) + w * 32),
+                      o);
+            uint32_t nan = 0;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) nan |= (uint32_t)(o[k] != o[k]) << k;
+            const uint32_t any = seen[0][w] | seen[1][w];
+            for (uint32_t left = any; left; left &= left - 1) {
+                const int b = __ffs(left) - 1, d = half * (HD / 2) + w * 32 + b;
+                const float v = odd_value((seen[0][w] >> b & 1u) | (seen[1][w] >> b & 1u) << 1);
+                if (a.splits > 1) part[d] = v;
+                else dst[d] = Elem<T>::from_f(v);
+            }
+            const uint32_t left = settle ? nan & ~any : 0u;
+            open[(half * HW + w) * C::ROWS + x.id] = left;
+            redo |= left != 0;
+        }
+    }
+    if (!softmax_or<TH>(redo)) return;
+
+    // ---- once more, 64 dims at a time
+    constexpr int KT = 64, NT = 8;  // keys of a tile, 8-dim columns
+    uint8_t* kt = smem + L.v;       // [HD/64][KT][64], 128-byte swizzle
+    uint8_t* vt = kt + KT * HD * 2;  // [KT][64], swizzled
+    static_assert(KT * HD * 2 + KT * 128 <= C::NS * C::KBYTES && 2 * HD * W * 4 + KW * C::ROWS * 4 <= C::NS * C::KBYTES, "fits the stages");
+    const int gq = lane >> 2, qq = lane & 3, row0 = warp * 16;
+    const Row rows[2] = {row_of<HD>(a, rt, hk, row0 + gq, n_keys), row_of<HD>(a, rt, hk, row0 + gq + 8, n_keys)};
+    float slope[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) slope[i] = a.p.f.slopes && rows[i].mine ? a.p.f.slopes[rows[i].head] * kLog2E : 0.f;
+    const bool capped = a.p.f.cap > 0.f;
+    const float scale2 = a.p.f.scale * kLog2E, cap2 = a.p.f.cap * kLog2E, inv_cap = capped ? a.p.f.scale / a.p.f.cap : 0.f;
+    const uint32_t qt = smem_u32(smem + L.q) + (uint32_t)(row0 >> 7) * C::QBYTES;
+    const uint32_t q_row = (uint32_t)((row0 & 127) + (lane & 7) + ((lane >> 3) & 1) * 8), x7 = (uint32_t)(lane & 7);
+#pragma unroll 1
+    for (int part = 0; part < HD / 64; ++part) {
+        uint32_t todo[2][2];  // outputs of the two rows in these dims
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) todo[i][w] = open[(part * 2 + w) * C::ROWS + rows[i].id];
+        const bool work = __any_sync(0xffffffffu, todo[0][0] | todo[0][1] | todo[1][0] | todo[1][1]);
+        if (!softmax_or<TH>(work)) continue;
+        float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+#pragma unroll 1
+        for (int k0 = key_lo; k0 < key_hi; k0 += KT) {
+            softmax_or<TH>(false);  // the last tile is read
+            for (int c = tid; c < KT * CH; c += TH) {
+                const int j = c / CH, d = c % CH * 8;
+                const uint4 v = k0 + j < key_hi ? value_at(a.p.k_pages, k0 + j, d) : make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(kt + swz(KT, j, d)) = v;
+            }
+            for (int c = tid; c < KT * 8; c += TH) {
+                const int j = c / 8, d = c % 8 * 8;
+                uint4 v = k0 + j < key_hi ? value_at(a.p.v_pages, k0 + j, part * 64 + d) : make_uint4(0, 0, 0, 0);
+                finite_only<T>(v);
+                *reinterpret_cast<uint4*>(vt + swz(KT, j, d)) = v;
+            }
+            softmax_or<TH>(false);
+            if (!work) continue;
+#pragma unroll 1
+            for (int jb = 0; jb < KT; jb += 16) {
+                float c[2][4];  // c[nt][0..1]: row gq, keys k0 + jb + 8 nt + 2 qq + {0, 1}; c[nt][2..3]: row gq + 8
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
+#pragma unroll 2
+                for (int ks = 0; ks < HD / 16; ks += 2) {
+                    uint32_t q0[4], q1[4];
+                    const uint32_t qo = qt + ((uint32_t)(ks >> 2) * 128u + q_row) * 128u, y = (uint32_t)(ks & 3) * 2u + (uint32_t)(lane >> 4);
+                    ldsm4(qo + ((y ^ x7) << 4), q0[0], q0[1], q0[2], q0[3]);
+                    ldsm4(qo + (((y + 2u) ^ x7) << 4), q1[0], q1[1], q1[2], q1[3]);
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        uint32_t b0, b1, b2, b3;
+                        ldsm4(smem_u32(kt) + (uint32_t)((ks >> 2) * KT + jb + nt * 8 + (lane & 7)) * 128u +
+                                  ((((uint32_t)(ks & 3) * 2u + (uint32_t)(lane >> 3)) ^ x7) << 4),
+                              b0, b1, b2, b3);
+                        mma16<T>(c[nt], q0, b0, b1);
+                        mma16<T>(c[nt], q1, b2, b3);
+                    }
+                }
+                uint32_t ph[4], pl[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {  // the two rows
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int j = k0 + jb + nt * 8 + qq * 2 + e;
+                            const float z = c[nt][2 * i + e];
+                            float y = capped ? cap2 * tanhf(z * inv_cap) : z * scale2;
+                            y = fmaf(-slope[i], fabsf((float)(rows[i].pos - j)), y);
+                            c[nt][2 * i + e] = j >= rows[i].lo && j < min(rows[i].hi, key_hi) ? y : -INFINITY;
+                            top = fmaxf(top, c[nt][2 * i + e]);
+                        }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), m[i]);
+                    const float u = top == -INFINITY ? 0.f : top, f = ex2(m[i] - u);
+                    m[i] = top;
+                    l[i] *= f;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        o[n][2 * i] *= f;
+                        o[n][2 * i + 1] *= f;
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const float p0 = ex2(c[nt][2 * i] - u), p1 = ex2(c[nt][2 * i + 1] - u);
+                        l[i] += p0 + p1;
+                        split_p<T>(p0, p1, ph[2 * nt + i], pl[2 * nt + i]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    uint32_t b0, b1, b2, b3;
+                    ldsm4_t(smem_u32(vt) + (uint32_t)(jb + (lane & 7) + ((lane >> 3) & 1) * 8) * 128u +
+                                ((((uint32_t)n + (uint32_t)(lane >> 4)) ^ x7) << 4),
+                            b0, b1, b2, b3);
+                    mma16<T>(o[n], ph, b0, b1);
+                    mma16<T>(o[n + 1], ph, b2, b3);
+                    mma16<T>(o[n], pl, b0, b1);
+                    mma16<T>(o[n + 1], pl, b2, b3);
+                }
+            }
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (a.splits > 1) part[d + i] = acc[i];
-            else dst[d + i] = Elem<T>::from_f(acc[i] * inv);
+        for (int i = 0; i < 2; ++i) {
+            float sum = l[i] + __shfl_xor_sync(0xffffffffu, l[i], 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const int64_t at = ((int64_t)blockIdx.z * a.p.r.n_tokens + rows[i].token) * a.p.n_heads + rows[i].head;
+            T* dst = reinterpret_cast<T*>(a.p.out) + (int64_t)rows[i].token * a.p.out_stride + (int64_t)rows[i].head * HD;
+            float f = sum == 0.f ? 0.f : 1.f / sum;
+            if (a.splits > 1 && (todo[i][0] | todo[i][1])) {  // in the partial's units: against its maximum and sum
+                const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[at];
+                f = f * ml.y;
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = n * 8 + qq * 2 + e;
+                    if (!(todo[i][d / 32] >> (d % 32) & 1u)) continue;
+                    const float v = o[n][2 * i + e] * f;
+                    if (a.splits > 1) a.part_o[at * HD + part * 64 + d] = v;
+                    else dst[part * 64 + d] = Elem<T>::from_f(v);
+                }
         }
     }
 }
@@ -298,24 +531,15 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
 
     const RowTile rt = find_rows<C::ROWS>(a, blockIdx.x / a.p.n_kv);
     if (rt.seq < 0) return;  // the whole block
-    const int s = rt.seq;
-    const int n_rows = (rt.t1 - rt.t0) * a.group - rt.row0;  // rows of the sequence from the tile's first on
 
     // ---- this thread's row (softmax threads): token, head, position, keys [lo, hi)
     const int kv_len = rt.kv_len;
     const int32_t* table = rt.row >= 0 && rt.row < a.p.r.table_rows ? a.p.r.table + (size_t)rt.row * a.p.r.pt_stride : nullptr;
     const int n_keys = table ? min(max(kv_len, 0), a.p.r.pt_stride * kPageTokens) : 0;
-    int token = 0, head = 0, pos = 0, lo = 0, hi = 0;
-    // (softmax warps 8 q + 4 half + quarter: the row of lane l is 128 q + 32 quarter + l)
-    const int row_id = (warp >> 3) * 128 + (warp & 3) * 32 + lane;
-    const bool mine = warp < C::SW && row_id < n_rows;
-    if (mine) {
-        const int r = rt.row0 + row_id;
-        token = rt.t0 + r / a.group;
-        head = hk * a.group + r % a.group;
-        pos = kv_len - (rt.t1 - token);
-        key_range(a.p.f, s, token, pos, n_keys, lo, hi);
-    }
+    const Row own = row_of<HD>(a, rt, hk, warp < C::SW ? (warp >> 3) * 128 + (warp & 3) * 32 + lane : C::ROWS, n_keys);
+    const bool mine = own.mine;
+    const int token = own.token, head = own.head;
+    int pos = own.pos, lo = own.lo, hi = own.hi;
     // ---- Q rows into shared memory (rows past the end are zero): the two warps of 32 rows take 16 each, in copies that
     // run on while the block comes up
     if (warp < C::SW) {
@@ -388,12 +612,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, (uint32_t)misc[0], 0);
     const int key_lo = range[0], key_hi = range[1];  // keys some row of the CTA sees
-    int j0 = key_hi > key_lo ? key_lo / BN : 0, j1 = key_hi > key_lo ? (key_hi + BN - 1) / BN : 0;
-    if (a.splits > 1) {
-        const int per = (j1 - j0 + a.splits - 1) / a.splits;
-        j0 = min(j1, j0 + (int)blockIdx.z * per);
-        j1 = min(j1, j0 + per);
-    }
+    int j0, j1;
+    key_tiles<BN>(a, key_lo, key_hi, j0, j1);
     const int nt = __shfl_sync(0xffffffffu, j1 - j0, 0);  // key tiles of this CTA
 
     // a tile from its pages (lane l holds the pool row of page l), one lane issuing
@@ -411,6 +631,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         __syncwarp();
     };
     if (NQ == 2 && warp >= C::SW) regs_dec<regs_other(CAP)>();
+    bool more = false;  // an output is not finite
     // from the last tile to the first: under a distance bias the largest scores come first, so the maximum
     // does not grow with every tile
     auto tile = [&](int it) { return j0 + nt - 1 - it; };
@@ -755,7 +976,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             good = __all_sync(0xffffffffu, pipe_wait(&o_full[q], 0, stop));
             tc_fence_after();
         }
-        float odd = 0.f;  // NaN once one of the thread's outputs is a NaN or an infinity
+        float sum = 0.f;  // NaN once one of the thread's outputs is a NaN or an infinity
         if (a.splits > 1) {
             const int64_t row = ((int64_t)blockIdx.z * a.p.r.n_tokens + token) * a.p.n_heads + head;
             // (a row that saw none of these keys has no part in the join, whatever zero times V came to)
@@ -766,7 +987,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                     float o[32];
                     tmem_ld32(t_lane + C::O_COL + (uint32_t)(q * HD + c), o);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) odd = fmaf(o[k], 0.f, odd);
+                    for (int k = 0; k < 32; ++k) sum = fmaf(o[k], 0.f, sum);
                     if (mine)
 #pragma unroll
                         for (int k = 0; k < 32; k += 4)
@@ -784,7 +1005,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 if (nt > 0) {
                     tmem_ld32(t_lane + C::O_COL + (uint32_t)(q * HD + c), o);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) odd = fmaf(o[k], 0.f, odd);
+                    for (int k = 0; k < 32; ++k) sum = fmaf(o[k], 0.f, sum);
                 }
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
@@ -803,15 +1024,23 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 }
             }
         }
-        // A NaN or an infinity in V meets rows of its tile that do not see it with a probability of zero, and
-        // zero times it is NaN.  A thread with such outputs makes them once more, from the keys its row sees alone.
-        // (Taking such values out of V before the MMAs read it costs each tile with a partly seen key some 3,000
-        // cycles: 23 -> 37 us for short prompts.)
-        const bool again = mine && odd != 0.f && l == l && l != 0.f;
-        if (__any_sync(0xffffffffu, again)) odd_rows<HD, T>(a, row_id, half, j0 * BN, j1 * BN, again, m, 1.f / l);
+        // ---- where the block ends, as a rule
+        const bool settle = mine && l == l && l != 0.f;  // the row has keys here
+        tc_fence_before();
+        more = __syncthreads_or(sum != 0.f && settle);
+        if (more) {
+            tc_fence_after();
+            settle_odd<HD, T>(a, smem, tmem, settle);
+        }
     }
-    tc_fence_before();
-    __syncthreads();
+    if (warp >= C::SW) {
+        tc_fence_before();
+        more = __syncthreads_or(false);
+    }
+    if (more) {
+        tc_fence_before();
+        __syncthreads();
+    }
     if (warp == kMmaWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");

@@ -134,6 +134,99 @@ def test_decode_infinity_counts_however_small_its_weight(length, dtype):
     same_odd_values(out, want, ref, tol)
 
 
+FORMS = {
+    "plain": {},
+    "cap": dict(cap=30.0),
+    "bias": dict(bias=True),
+    "window": dict(window=300),
+    "prefix": dict(prefix=True),
+    "docs": dict(docs=190),
+    "all": dict(cap=8.0, bias=True, window=700, prefix=True, docs=411, scale=0.2),
+}
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("hd, dtype", [(64, "bf16"), (128, "f16"), (256, "bf16")])
+@pytest.mark.parametrize("max_len", [0, 1 << 20])  # the second: keys divided over CTAs
+def test_prefill_settles_the_odd_values_of_every_mask(max_len, hd, dtype, form):
+    # rows that share tiles with an odd value and do not see it are computed again, the others take it, under every mask
+    heads, nkv = 4, 1
+    c = Cache([(500, 700), (3, 400), (130, 130)], nkv, hd, dtype, seed=34)
+    c.max_len = max_len or c.max_len
+    f = forms(c, heads, **FORMS[form])
+    if f["prefix"] is not None:
+        f["prefix"] = np.array([390, 399, 77], np.int32)
+    q = queries(c, heads)
+    ref, tol = attend(c, q, heads, **f)
+    d = c.dev()
+    clean = launch(c, d, q, heads, "prefill", f)
+    within(clean, ref, tol)
+    want = np.zeros((c.tokens, heads, hd))
+    for s, n in enumerate([700, 400, 130]):
+        for i, j in enumerate([0, 1, 2, 60, 61, 129, 128, 397, 398, 399, 400, 512, 600, 699]):
+            if j < n and (s, i) != (0, 0):
+                dim, value = (11 * j + 29 * i) % hd, ODD[i % 3]
+                put(c, d["v"], s, j, 0, dim, value)
+                with np.errstate(invalid="ignore"):
+                    want[c.starts[s]:c.starts[s] + c.seqs[s][0], :, dim][sees(c, s, j, f)] += value
+    same_odd_values(launch(c, d, q, heads, "prefill", f), want, ref, tol)
+
+
+@pytest.mark.parametrize("dtype, hd", [("bf16", 64), ("f16", 128)])
+def test_prefill_infinity_counts_however_small_its_weight(dtype, hd):
+    c = Cache([(40, 200)], 1, hd, dtype, seed=35)
+    c.K[0][:] = 0.0
+    c.K[0][20:22] = -50.0
+    d = c.dev()
+    for p in range(13):
+        m = min(16, 200 - p * 16)
+        d["k"][int(c.table[c.rows[0], p]), :, :m] = c.K[0][p * 16:p * 16 + m].transpose(0, 1).cuda()
+    q = torch.ones(40, 2, hd, dtype=DT[dtype])
+    f = forms(c, 2)
+    ref, tol = attend(c, q, 2, **f)
+    put(c, d["v"], 0, 20, 0, 3, float("inf"))
+    put(c, d["v"], 0, 21, 0, 40, -float("inf"))
+    want = np.zeros((40, 2, hd))
+    want[..., 3], want[..., 40] = np.inf, -np.inf
+    same_odd_values(launch(c, d, q, 2, "prefill", f), want, ref, tol)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("where", ["first", "middle", "everywhere"])
+def test_prefill_with_odd_values_takes_a_few_times_its_time(where, hd):
+    # (what every row sees is settled by one reading of V; the rows of one tile before the middle are computed again)
+    n, heads, nkv = 2048, 16, 4
+    c = Cache([(n, n)], nkv, hd, "bf16", seed=36)
+    d, f, q = c.dev(), forms(c, heads), queries(c, heads).cuda()
+    out = torch.empty(n, heads, hd, dtype=torch.bfloat16, device="cuda")
+
+    def fastest():
+        fm, best = ti.AttnForm(), 1e9
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            ti.check(ti.lib().ti_op_paged_prefill(C.byref(d["kv"]), C.byref(d["batch"]), C.byref(fm), q.data_ptr(),
+                                                  heads * hd, heads, out.data_ptr(), heads * hd, stream()))
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    clean = launch(c, d, q, heads, "prefill", f)
+    base = fastest()
+    for j in {"first": [0], "middle": [n // 2 + 13], "everywhere": range(n)}[where]:
+        for h in range(nkv):
+            put(c, d["v"], 0, j, h, 7, float("nan"))
+    took = fastest()
+    torch.cuda.synchronize()
+    got, first = out.float(), {"first": 0, "middle": n // 2 + 13, "everywhere": 0}[where]
+    assert got[first:, :, 7].isnan().all() and not got[:first, :, 7].isnan().any()
+    got[:, :, 7], rest = 0, clean.float()
+    rest[:, :, 7] = 0
+    assert torch.equal(got, rest)
+    assert took < 8 * base, f"{took:.3f} ms against {base:.3f}"
+
+
 @pytest.mark.parametrize("hd, dtype", [(64, "bf16"), (128, "f16"), (256, "bf16")])
 def test_prefill_join_keeps_the_odd_values_of_a_share_without_weight(hd, dtype):
     # keys divided over CTAs, and a distance bias that leaves the first share no weight in fp32: its NaN still counts

@@ -28,6 +28,9 @@ template <>
 struct Elem<__nv_bfloat16> {
     static constexpr uint32_t kUmmaFmt = 1;  // tcgen05 kind::f16 operand format
     static constexpr uint32_t kExp = 0x7f80u;  // the exponent's bits: all set in an infinity or a NaN
+    // Probabilities go into products as 2^kTop p: f16 has 15 powers of two above 1 and only 24 below, and a long
+    // cache's weights may all lie under 2^-24 of the largest.  (The factor leaves with the sum it is divided by.)
+    static constexpr float kTop = 0.f;
     static TI_DEVICE_INLINE float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
     static TI_DEVICE_INLINE __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
     static TI_DEVICE_INLINE float lo(uint32_t u) { return __uint_as_float(u << 16); }
@@ -42,6 +45,7 @@ template <>
 struct Elem<__half> {
     static constexpr uint32_t kUmmaFmt = 0;
     static constexpr uint32_t kExp = 0x7c00u;
+    static constexpr float kTop = 15.f;
     static TI_DEVICE_INLINE float to_f(__half v) { return __half2float(v); }
     static TI_DEVICE_INLINE __half from_f(float v) { return __float2half_rn(v); }
     static TI_DEVICE_INLINE float lo(uint32_t u) { return __half2float(__ushort_as_half((unsigned short)(u & 0xffffu))); }

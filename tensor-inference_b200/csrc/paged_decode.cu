@@ -401,8 +401,8 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                 mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
                 mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
                 const float n0 = fmaxf(m0, mx0);
-                const float u0 = n0 == -INFINITY ? 0.f : n0;
-                const float al0 = ex2(m0 - u0);
+                const float u0 = (n0 == -INFINITY ? 0.f : n0) - Elem<T>::kTop;
+                const float al0 = n0 == -INFINITY ? 0.f : ex2(m0 - n0);
                 m0 = n0;
                 float s0 = 0.f;
 #pragma unroll
@@ -419,8 +419,8 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
                     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
                     const float n1 = fmaxf(m1, mx1);
-                    const float u1 = n1 == -INFINITY ? 0.f : n1;
-                    al1 = ex2(m1 - u1);
+                    const float u1 = (n1 == -INFINITY ? 0.f : n1) - Elem<T>::kTop;
+                    al1 = n1 == -INFINITY ? 0.f : ex2(m1 - n1);
                     m1 = n1;
                     float s1 = 0.f;
 #pragma unroll
@@ -443,7 +443,8 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                         }
                     }
                 }
-                // ---- P.V, P = hi + lo in 16 bits: what the two drop is under 2^-16 of p (bf16) or 2^-22 (f16)
+                // ---- P.V, P = hi + lo in 16 bits: what the two drop is under 2^-16 of p (bf16) or 2^-22 (f16; under 2^-40
+                // of the largest p where that is more: half of f16's smallest step, 2^-24, with p scaled by 2^15)
                 uint32_t ph[4], pl[4];
                 split_p<T>(c[0][0], c[0][1], ph[0], pl[0]);
                 split_p<T>(c[1][0], c[1][1], ph[2], pl[2]);

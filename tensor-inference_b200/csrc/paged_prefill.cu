@@ -17,10 +17,13 @@
 //                   (N-major: a V row is 64 dims of one key)
 // K and V tiles are assembled from pages by TMA, a 2 KB box per page and 64 dims.
 // The output stays in TMEM; it is rescaled only when a row's maximum has grown by more than
-// 2^8 since the last time (P then stays under 2^8, far from overflow in either type), which
-// is rare after the first tiles.  P is rounded once to the operand type, half a step of
-// it (2^-8 of p for bf16, 2^-11 for f16) on each term, as the product's inputs must be; the
-// sum is that of the rounded values, so that a row on few keys, or with one large weight, does
+// 2^8 (bf16) or 2^4 (f16) since the last time, which is rare after the first tiles.  P then stays under
+// 2^8, far from overflow; in f16 it is scaled by 2^11 besides and stays under 2^15, so that weights down
+// to 2^-25 of the largest are normal numbers and smaller ones off by at most 2^-36 of it (8,192 f16
+// tokens at head_dim 128 / 64 / 256: 514 / 449 / 511 us with a lag of 2^8 and weights normal to 2^-21,
+// 529 / 460 / 535 with 2^4, 536 / 464 / 544 with 2^2 and 2^-27).  P is rounded once to the operand type,
+// half a step of it (2^-8 of p for bf16, 2^-11 for f16) on each term, as the product's inputs must be;
+// the sum is that of the rounded values, so that a row on few keys, or with one large weight, does
 // not keep their rounding (the result's error against 64 bits is 1.1 to 1.4 times that of a result
 // rounded once; with the sum of the unrounded ones 1.3 to 1.5, at 4 to 8% less time).
 //
@@ -445,7 +448,7 @@ TI_DEVICE_INLINE void settle_odd(const PreArgs& a, uint8_t* smem, uint32_t tmem,
                         }
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), m[i]);
-                    const float u = top == -INFINITY ? 0.f : top, f = ex2(m[i] - u);
+                    const float f = top == -INFINITY ? 0.f : ex2(m[i] - top), u = (top == -INFINITY ? 0.f : top) - Elem<T>::kTop;
                     m[i] = top;
                     l[i] *= f;
 #pragma unroll
@@ -792,6 +795,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
+        constexpr float kLag = Elem<T>::kTop > 0.f ? 4.f : 8.f;  // powers of two that the maximum may lag behind
         const float scale2 = a.p.f.scale * kLog2E;
         const float u1 = CAP ? a.p.f.scale / a.p.f.cap : 0.f;  // u = u1 q.k
         const float cap2 = a.p.f.cap * kLog2E;
@@ -904,7 +908,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 pair_bar();
                 mx = fmaxf(mx, *xrow(it & 1, half ^ 1));
                 // ---- lazily rescaled maximum
-                bool grow = mx > m + 8.f;  // (m = -inf: the first keys of the row)
+                bool grow = mx > m + kLag;  // (m = -inf: the first keys of the row)
                 if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
                     if (NQ == 1 && it > 0) {  // with two streams s_full(it) already says that P V (it - 1) is done
                         pipe_wait(&pv_done[0], (it - 1) & 1, stop);
@@ -926,7 +930,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 }
                 if (grow) m = mx;
             }
-            const float u = m == -INFINITY ? 0.f : m;
+            const float u = (m == -INFINITY ? 0.f : m) - (Elem<T>::kTop > 0.f ? Elem<T>::kTop - kLag : 0.f);
             // (scalar sums at head_dim 128: 474 against 486 us for 8,192 causal tokens, capped 470 against 493; packed
             // elsewhere: 414 against 424 at 64)
             float2 sum = dup2(0.f);

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import ti_b200 as ti
-from paged_ref import DT, Cache, attend
+from paged_ref import DT, FLOOR, Cache, attend
 from test_gpu_paged_ops import queries, run_attention, stream, within
 
 pytestmark = pytest.mark.gpu
@@ -242,3 +242,34 @@ def test_prefill_join_keeps_the_odd_values_of_a_share_without_weight(hd, dtype):
     want = np.zeros((20, heads, hd))
     want[..., 17] = np.nan
     same_odd_values(launch(c, d, q, heads, "prefill", f), want, ref, tol)
+
+
+# ------------------------------------------------------------------ weights small beside the largest
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("gap", [10.0, 17.5, 19.0])  # weights of e^-10, 2^-25.2 and 2^-27.4 of the largest
+@pytest.mark.parametrize("entry, new, hd, max_len", [("decode", 1, 64, 0), ("decode", 1, 128, 1), ("prefill", 3, 64, 0),
+                                                     ("prefill", 3, 128, 1), ("prefill", 3, 256, 1)])
+def test_many_small_weights_beside_a_large_one(entry, new, hd, max_len, gap, dtype):
+    # one key takes nearly all the weight and its value is zero: the result is what the other 20,000 have together
+    # (decode with max_len 1 runs in one CTA, so that warps meet many keys after the large one)
+    n = 20000
+    c = Cache([(new, n)], 1, hd, dtype, seed=38)
+    c.max_len = max_len or c.max_len
+    c.K[0][:] = 0.0
+    c.K[0][40] = gap / hd ** 0.5  # q of ones: a score of hd k / sqrt(hd)
+    c.V[0] = c.V[0].abs() + 0.5
+    c.V[0][40] = 0.0
+    at = c.table[c.rows[0]].long()
+    pad = 16 * len(at) - n
+    for pool, rows in ((c.k, c.K[0]), (c.v, c.V[0])):
+        rows = torch.cat([rows, torch.zeros(pad, 1, hd, dtype=rows.dtype)])
+        pool[at] = rows.view(-1, 16, 1, hd).transpose(1, 2)
+    q = torch.ones(new, 2, hd, dtype=DT[dtype])
+    f = forms(c, 2)
+    ref, tol = attend(c, q, 2, **f)
+    # attend allows each key half a smallest step of the type beside a largest p of 1; here it is of 2^15 p (decode: two
+    # terms) or of 2^11 p at least (prefill)
+    values = c.V[0][:, 0].double().abs().sum(0).numpy()
+    tol = tol - FLOOR[dtype] * (1 + values) + FLOOR[dtype] * (1 + values * 2.0 ** (-15 if entry == "decode" else -11))
+    assert (tol < 0.02 * ref).all() or dtype == "bf16"
+    within(launch(c, c.dev(decode=entry == "decode"), q, 2, entry, f), ref, tol)

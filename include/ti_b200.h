@@ -59,6 +59,10 @@ ti_status ti_shutdown(void);
  * both gave up and set their error bits; waited_us[0..1] (may be NULL) = how
  * long each waited.  TI_ERR_STATE when a wait did not report giving up. */
 ti_status ti_selftest_waits(int device, int limit_us, double* waited_us);
+/* For tests: the following ti_op_paged_prefill / ti_op_paged_decode calls of the process run as if, in every
+ * block, a wait had given up at this step of its key loop (0 .. ; blocks with fewer steps are not
+ * affected).  -1 (the default): as usual. */
+ti_status ti_selftest_paged_stop(int step);
 
 /* ================================================================= device
  * replaces tensor::backend::Device (include/tensor/backend/device.hpp:10-42,
@@ -157,7 +161,9 @@ ti_status ti_op_paged_attention_noalloc(const void* qkv, int batch, int n_heads,
  * be captured into graphs; captured graphs share no scratch.  What arrays on the
  * device say is checked there: a token without a sequence, a position outside
  * the page table, and a row or page id out of range read as "no such key" or
- * are skipped, not reported. */
+ * are skipped, not reported.  Every wait inside the attention kernels, for their own
+ * copies and products, is bounded (2 s); one that runs out ends its block's work, and the
+ * rows that the block did not finish are NaN. */
 
 /* Rotary positions on one to four axes (time, height, width ...).  Pair
  * (i, i + rot_dim/2) of the first rot_dim dimensions of a head turns by

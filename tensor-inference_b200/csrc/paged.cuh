@@ -12,7 +12,7 @@ constexpr int kPageTokens = 16;
 constexpr float kLog2E = 1.4426950408889634f;
 
 // Bounded wait of a pipeline role: false once `stop` is set by a wait that gave up (its own or another
-// role's).  The flag is read only after a poll has failed: while MMAs stream operands out of shared
+// role's).  A role that gets false stops, and the rows it was for become NaN.  The flag is read only after a poll has failed: while MMAs stream operands out of shared
 // memory every other access to it takes some 200 cycles.
 TI_DEVICE_INLINE bool pipe_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -228,6 +228,7 @@ struct PagedAttn {
     const void* v_pages;
     int n_heads, n_kv, hd, dtype;
     int max_len;
+    int stop_at;  // step at which the warp that loads K stops, as after a wait that gave up; -1: none (ti_selftest_paged_stop)
 };
 // Pages as a 3-D tensor of 16-bit elements [hd/64][rows][64]: one box is the 16 rows of a page and
 // kv head in `parts` of their 64-dim parts, stored [part][16][64] with 128-byte swizzle.

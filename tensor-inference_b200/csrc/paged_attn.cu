@@ -1,5 +1,6 @@
 // paged_attn.cu — entry points of attention over the paged cache (prefill and decode forms).
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "paged.cuh"
@@ -26,6 +27,8 @@ bool make_tmap_pages(CUtensorMap* m, const void* base, int rows, int hd, int par
 }
 
 namespace {
+
+std::atomic<int> g_stop_at{-1};
 
 ti_status paged_args(const ti_paged_kv* kv, const ti_ragged* batch, const ti_attn_form* form, const void* q,
                      int64_t q_stride, int n_heads, void* out, int64_t out_stride, const char* who, PagedAttn* a) {
@@ -60,6 +63,7 @@ ti_status paged_args(const ti_paged_kv* kv, const ti_ragged* batch, const ti_att
     a->hd = hd;
     a->dtype = kv->dtype;
     a->max_len = std::max(1, batch->max_len);
+    a->stop_at = g_stop_at.load(std::memory_order_relaxed);
     return TI_OK;
 }
 
@@ -70,6 +74,12 @@ ti_status paged_args(const ti_paged_kv* kv, const ti_ragged* batch, const ti_att
 using namespace ti;
 
 extern "C" {
+
+ti_status ti_selftest_paged_stop(int step) {
+    TI_CHECK(step >= -1, TI_ERR_INVALID, "selftest_paged_stop: step %d", step);
+    g_stop_at.store(step, std::memory_order_relaxed);
+    return TI_OK;
+}
 
 ti_status ti_op_paged_prefill(const ti_paged_kv* kv, const ti_ragged* batch, const ti_attn_form* form, const void* q,
                               int64_t q_stride, int n_heads, void* out, int64_t out_stride, void* stream) {

@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         const CUtensorMap* tm = warp == kDecWarps ? &tk : &tv;
         const uint32_t half = warp == kDecWarps ? 0u : VOFF;
         int it = 0, issued = 0;
+        bool dead = false;  // a wait gave up: nothing more is requested
         segments([&](int, const SeqRange& x, int seg, int p0, int p1) {
             const int hk = seg / a.chunks;
             const int32_t* ids = x.row + x.pg0;
@@ -249,7 +250,9 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                     ahead = p + 32 + lane < p1 ? ids[p + 32 + lane] : 0;
                 }
                 const int id = __shfl_sync(0xffffffffu, cur, (i + lane) & 31);  // lane l: page p + l
-                if (!__all_sync(0xffffffffu, pipe_wait(&empty[slot], ((it / NS) & 1) ^ 1, stop))) continue;
+                if (half == 0u && it == a.p.stop_at) *stop = dead = true;
+                dead = dead || !__all_sync(0xffffffffu, pipe_wait(&empty[slot], ((it / NS) & 1) ^ 1, stop));
+                if (dead) continue;
                 // a page that does not exist reads as zeros: rows past the end of the pool
                 const int row = id >= 0 && id < a.p.r.n_pages ? (id * a.p.n_kv + hk) * kPageTokens : a.cache_rows;
                 const bool one = elect_one();
@@ -265,9 +268,10 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                 __syncwarp();
             }
         });
-        // copies in flight land before the block ends (they have, unless a wait gave up)
+        // copies in flight land before the block ends (they have, unless a wait gave up; then a stage may lack the other
+        // warp's half, and this one waits 0.1 s, by when its own are there)
         for (int i = max(0, issued - NS); i < issued; ++i)
-            if (!mbar_wait(&full[i % NS], (i / NS) & 1, nullptr, 0)) break;
+            if (!mbar_wait_for(&full[i % NS], (i / NS) & 1, nullptr, 0, kWaitNs / 20)) break;
         return;
     }
 
@@ -350,8 +354,11 @@ __global__ void __launch_bounds__(kDecThreads, 1)
             const int tok0 = (x.pg0 + p0 + st * CP) * kPageTokens;  // key of stage row 0
             const int rows = min(CP, p1 - p0 - st * CP) * kPageTokens;
             const int jlo = max(x.lo - tok0, 0), jhi = min(x.hi - tok0, rows);
-            const bool bad = !__all_sync(0xffffffffu, pipe_wait(&full[slot], (gi / NS) & 1, stop));
-            if (j0 + 16 > jlo && j0 < jhi && !bad) {  // warp-uniform
+            if (!__all_sync(0xffffffffu, pipe_wait(&full[slot], (gi / NS) & 1, stop))) {
+                l0 = l1 = __int_as_float(0x7fffffff);  // keys are missing: the rows are NaN; and the slot is not handed back
+                continue;
+            }
+            if (j0 + 16 > jlo && j0 < jhi) {  // warp-uniform
                 const bool edge = j0 < jlo || j0 + 16 > jhi;
                 if (edge) {
                     // unseen rows get probability 0: whatever their V holds must not enter

@@ -633,6 +633,10 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         }
         __syncwarp();
     };
+    // the copies of the last stages requested land before the block ends (they have, unless a wait gave up)
+    auto landed = [&](uint64_t* full, int issued) {
+        for (int i = max(0, issued - NS); i < issued; ++i) mbar_wait(&full[i % NS], (i / NS) & 1, nullptr, 0);
+    };
     if (NQ == 2 && warp >= C::SW) regs_dec<regs_other(CAP)>();
     bool more = false;  // an output is not finite
     // from the last tile to the first: under a distance bias the largest scores come first, so the maximum
@@ -640,19 +644,21 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
     auto tile = [&](int it) { return j0 + nt - 1 - it; };
     if (warp == kKWarp) {
         // ---------------------------------------------------------- K
+        int issued = 0;
         for (int it = 0; it < nt; ++it) {
             const int st = it % NS;
             const int page = tile(it) * C::PAGES + lane;
             const int id = lane < C::PAGES && page * kPageTokens < n_keys ? table[page] : -1;
             const int row = id >= 0 && id < a.p.r.n_pages ? (id * a.p.n_kv + hk) * kPageTokens : a.cache_rows;
-            if (!__all_sync(0xffffffffu, pipe_wait(&k_empty[st], ((it / NS) & 1) ^ 1, stop))) break;
+            if (it == a.p.stop_at) *stop = 1;
+            if (it == a.p.stop_at || !__all_sync(0xffffffffu, pipe_wait(&k_empty[st], ((it / NS) & 1) ^ 1, stop))) break;
             load_tile(smem + L.k + (uint32_t)st * C::KBYTES, &tk, row, &k_full[st]);
+            issued = it + 1;
         }
-        if (*stop)  // a wait gave up: copies in flight land before the block ends
-            for (int i = 0; i < NS; ++i) mbar_wait_for(&k_full[i], 0, nullptr, 0, 1000000);
+        landed(k_full, issued);
     } else if (warp == kVWarp) {
         // ---------------------------------------------------------- V
-        int edges = 0;
+        int edges = 0, issued = 0;
         for (int it = 0; it < nt; ++it) {
             const int st = it % NS, k0 = tile(it) * BN;
             const int page = tile(it) * C::PAGES + lane;
@@ -666,7 +672,10 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             uint8_t* vt = smem + L.v + (uint32_t)st * C::KBYTES;
             load_tile(vt, &tv, row, bar);
             if (edge) {
-                if (!__all_sync(0xffffffffu, pipe_wait(v_edge, edges & 1, stop))) break;
+                if (!__all_sync(0xffffffffu, pipe_wait(v_edge, edges & 1, stop))) {
+                    mbar_wait(v_edge, edges & 1, nullptr, 0);
+                    break;
+                }
                 ++edges;
                 const int lead = max(0, key_lo - k0), tail = min(BN, key_hi - k0);  // rows [lead, tail) are seen
                 for (int r = lane >> 3; r < lead + BN - tail; r += 4) {
@@ -679,9 +688,9 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&v_full[st]);
             }
+            issued = it + 1;
         }
-        if (*stop)
-            for (int i = 0; i < NS; ++i) mbar_wait_for(&v_full[i], 0, nullptr, 0, 1000000);
+        landed(v_full, issued);
     } else if (warp == kMmaWarp) {
         // ---------------------------------------------------------- MMA issue
         // One warp for both streams: a stream's P V and next scores are issued together, so the
@@ -975,17 +984,20 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         *xrow(nt & 1, half) = l;
         pair_bar();
         l += *xrow(nt & 1, half ^ 1);
+        // a wait of the row's threads or of the roles before them gave up: the row is NaN (a wait of the other half's thread
+        // shows in the flag, which it set before the barrier)
         bool good = true;
         if (nt > 0) {
-            good = __all_sync(0xffffffffu, pipe_wait(&o_full[q], 0, stop));
+            good = __all_sync(0xffffffffu, pipe_wait(&o_full[q], 0, stop)) && *stop == 0;
             tc_fence_after();
+            if (!good) l = __int_as_float(0x7fffffff);
         }
         float sum = 0.f;  // NaN once one of the thread's outputs is a NaN or an infinity
         if (a.splits > 1) {
             const int64_t row = ((int64_t)blockIdx.z * a.p.r.n_tokens + token) * a.p.n_heads + head;
             // (a row that saw none of these keys has no part in the join, whatever zero times V came to)
             if (mine && half == 0)
-                reinterpret_cast<float2*>(a.part_ml)[row] = nt > 0 && l != 0.f ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+                reinterpret_cast<float2*>(a.part_ml)[row] = !good ? make_float2(0.f, l) : nt > 0 && l != 0.f ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
             if (nt > 0 && good) {
                 for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                     float o[32];

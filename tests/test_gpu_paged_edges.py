@@ -273,3 +273,52 @@ def test_many_small_weights_beside_a_large_one(entry, new, hd, max_len, gap, dty
     tol = tol - FLOOR[dtype] * (1 + values) + FLOOR[dtype] * (1 + values * 2.0 ** (-15 if entry == "decode" else -11))
     assert (tol < 0.02 * ref).all() or dtype == "bf16"
     within(launch(c, c.dev(decode=entry == "decode"), q, 2, entry, f), ref, tol)
+
+
+# ------------------------------------------------------------------ waits that give up
+@pytest.mark.parametrize("hd, dtype", [(64, "bf16"), (128, "f16"), (256, "bf16")])
+@pytest.mark.parametrize("max_len", [0, 1 << 20])
+@pytest.mark.parametrize("step", [0, 2, 3])
+def test_prefill_rows_are_nan_where_a_wait_gives_up(step, max_len, hd, dtype):
+    # sequences of one key tile, of two and three, and of many
+    heads, nkv = 4, 1
+    seqs = [(30, 50), (20, 150), (700, 1500), (1, 1), (0, 9)]
+    c = Cache(seqs, nkv, hd, dtype, seed=39, pad_tokens=2)
+    c.max_len = max_len or c.max_len
+    d, f, q = c.dev(), forms(c, heads), queries(c, heads)
+    ref, tol = attend(c, q, heads, **f)
+    clean = launch(c, d, q, heads, "prefill", f)
+    real = int(c.starts[-1])
+    within(clean[:real], ref[:real], tol[:real])
+    try:
+        ti.check(ti.lib().ti_selftest_paged_stop(step))
+        out = launch(c, d, q, heads, "prefill", f)
+    finally:
+        ti.check(ti.lib().ti_selftest_paged_stop(-1))
+    lost = out[:real].isnan().any(-1)
+    assert torch.equal(out[:real].isnan().all(-1), lost)         # whole rows
+    assert torch.equal(out[:real][~lost], clean[:real][~lost])    # and the others as ever
+    s0, s1, s2 = (int(x) for x in c.starts[1:4])
+    assert lost.all() if step == 0 else not lost[:s0].any()
+    assert lost[s1:s2].any() or max_len  # (divided over CTAs, two key tiles may be all that a block has)
+    assert (out[real:] == 3.0).all()
+    assert torch.equal(launch(c, d, q, heads, "prefill", f), clean)
+
+
+@pytest.mark.parametrize("hd, dtype", [(64, "f16"), (128, "bf16"), (256, "f16")])
+@pytest.mark.parametrize("heads, lens, step", [(4, [900], 0), (4, [5000, 40, 700], 0), (12, [5000, 40, 700], 1), (4, [60000], 5)])
+def test_decode_rows_are_nan_where_a_wait_gives_up(heads, lens, step, hd, dtype):
+    c = Cache([(1, n) for n in lens], 1, hd, dtype, seed=40)
+    d, f, q = c.dev(decode=True), forms(c, heads), queries(c, heads)
+    ref, tol = attend(c, q, heads, **f)
+    clean = launch(c, d, q, heads, "decode", f)
+    within(clean, ref, tol)
+    try:
+        ti.check(ti.lib().ti_selftest_paged_stop(step))
+        out = launch(c, d, q, heads, "decode", f)
+    finally:
+        ti.check(ti.lib().ti_selftest_paged_stop(-1))
+    lost = out.isnan().any(-1)
+    assert torch.equal(out.isnan().all(-1), lost) and torch.equal(out[~lost], clean[~lost])
+    assert lost[0].all()
+    assert torch.equal(launch(c, d, q, heads, "decode", f), clean)

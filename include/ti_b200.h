@@ -159,9 +159,13 @@ ti_status ti_op_paged_attention_noalloc(const void* qkv, int batch, int n_heads,
  * and `stream` is a stream of that device (NULL = its legacy default stream).
  * They allocate nothing but stream-ordered scratch, synchronise nothing and may
  * be captured into graphs; captured graphs share no scratch.  What arrays on the
- * device say is checked there: a token without a sequence, a position outside
- * the page table, and a row or page id out of range read as "no such key" or
- * are skipped, not reported.  Every wait inside the attention kernels, for their own
+ * device say is checked there, not reported: a token without a sequence is
+ * skipped; a position outside the page table is skipped by the append and no key to
+ * the attention, as is every position of a sequence whose row is out of range; a page id
+ * out of range is skipped by the append and reads as 16 positions of zeros
+ * in K and V to the attention, which take their share of the weight (a score of
+ * 0 less the distance bias).  So a page that was given back is not marked by a bad id:
+ * leave it out by sliding_window or doc_start.  Every wait inside the attention kernels, for their own
  * copies and products, is bounded (2 s); one that runs out ends its block's work, and the
  * rows that the block did not finish are NaN. */
 

@@ -322,3 +322,27 @@ def test_decode_rows_are_nan_where_a_wait_gives_up(heads, lens, step, hd, dtype)
     assert torch.equal(out.isnan().all(-1), lost) and torch.equal(out[~lost], clean[~lost])
     assert lost[0].all()
     assert torch.equal(launch(c, d, q, heads, "decode", f), clean)
+
+
+# ------------------------------------------------------------------ pages that do not exist
+@pytest.mark.parametrize("form", ["plain", "cap", "bias", "all"])
+@pytest.mark.parametrize("hd, dtype", [(64, "f16"), (128, "bf16"), (256, "f16")])
+@pytest.mark.parametrize("entry, max_len", [("decode", 0), ("prefill", 0), ("prefill", 1 << 20)])
+def test_pages_that_do_not_exist_are_zeros_that_take_weight(entry, max_len, hd, dtype, form):
+    # with every real score far below zero the zeros take most of the weight
+    heads = 4
+    seqs = [(1, 600), (1, 33)] if entry == "decode" else [(150, 600), (33, 33)]
+    c = Cache(seqs, 1, hd, dtype, seed=41)
+    c.max_len = max_len or c.max_len
+    for s, (_, n) in enumerate(seqs):
+        c.K[s] = -c.K[s].abs()
+        for p in range(-(-n // 16)):
+            m = min(16, n - p * 16)
+            c.k[int(c.table[c.rows[s], p]), :, :m] = c.K[s][p * 16:p * 16 + m].transpose(0, 1)
+    for s, p, bad in ((0, 0, -1), (0, 9, c.n_pages), (0, 37, 2**31 - 1), (1, 1, -2**31)):
+        c.table[c.rows[s], p] = bad
+        c.K[s][p * 16:p * 16 + 16] = 0
+        c.V[s][p * 16:p * 16 + 16] = 0
+    q, f = queries(c, heads).abs(), forms(c, heads, **FORMS[form])
+    ref, tol = attend(c, q, heads, **f)
+    within(launch(c, c.dev(decode=entry == "decode"), q, heads, entry, f), ref, tol)

@@ -50,7 +50,7 @@ int ti_version(void); /* major*10000 + minor*100 + patch */
 ti_status ti_init(int* n_devices);
 /* Release what the library holds outside engines, PKM routers and GGUF files:
  * the ops' cached RoPE tables and the unused blocks of every device's
- * stream-ordered pool.  Call with no op in flight; the library stays usable. */
+ * stream-ordered pool and of the scratch pool that the paged operators keep there.  Call with no op in flight; the library stays usable. */
 ti_status ti_shutdown(void);
 /* Health check of the bounded device waits that guard every wait on another
  * CTA, kernel or rank (no counterpart in the reference, which never waits on
@@ -157,7 +157,9 @@ ti_status ti_op_paged_attention_noalloc(const void* qkv, int batch, int n_heads,
  * All pointers inside the structs and arguments are device pointers; the entries
  * select the device that holds `out` (or the pages), whatever device is current,
  * and `stream` is a stream of that device (NULL = its legacy default stream).
- * They allocate nothing but stream-ordered scratch, synchronise nothing and may
+ * They allocate nothing but stream-ordered scratch, from a pool of the library's own on
+ * the device (made by the first call, gone with cudaDeviceReset: not to be called after one; ti_shutdown
+ * gives its unused blocks back), synchronise nothing and may
  * be captured into graphs; captured graphs share no scratch.  What arrays on the
  * device say is checked there, not reported: a token without a sequence is
  * skipped; a position outside the page table is skipped by the append and no key to

@@ -2,13 +2,12 @@
 #include <atomic>
 #include <cmath>
 #include <cstring>
+#include <mutex>
 #include <string>
 
 #include "internal.h"
 
 namespace ti {
-
-cudaError_t pool_alloc(void** p, size_t bytes, int device, cudaStream_t s);
 
 static thread_local std::string g_last_error;
 
@@ -49,21 +48,41 @@ void rope_freqs(int head_dim, float theta, const ti_rope_scaling* sc, float* out
     }
 }
 
-// cudaMallocAsync from the device's default pool, whose release threshold the first
-// call raises: freed blocks stay in the pool across synchronisations (with the
-// default threshold of zero each first allocation after one maps memory anew, about
-// 400 us).  `device` is the current device.
-cudaError_t pool_alloc(void** p, size_t bytes, int device, cudaStream_t s) {
-    static std::atomic<bool> configured[64];
-    if (device >= 0 && device < 64 && !configured[device].load(std::memory_order_relaxed)) {
-        cudaMemPool_t pool;
-        if (cudaDeviceGetDefaultMemPool(&pool, device) == cudaSuccess) {
-            uint64_t thr = ~0ull;
-            cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &thr);
+// The operators' scratch comes from a pool of the library's own on each device, made by the first call there, which
+// keeps freed blocks across synchronisations (with a release threshold of zero each first allocation after one
+// maps memory anew, about 400 us).  The device's default pool, and its threshold, stay the caller's.
+static std::mutex g_scratch_mutex;
+static std::atomic<cudaMemPool_t> g_scratch_pool[64];
+
+// stream-ordered scratch; `device` is the current device
+cudaError_t scratch_alloc(void** p, size_t bytes, int device, cudaStream_t s) {
+    if (device < 0 || device >= 64) return cudaErrorInvalidDevice;
+    cudaMemPool_t pool = g_scratch_pool[device].load(std::memory_order_acquire);
+    if (!pool) {
+        std::lock_guard<std::mutex> lock(g_scratch_mutex);
+        pool = g_scratch_pool[device].load(std::memory_order_relaxed);
+        if (!pool) {
+            cudaMemPoolProps props{};
+            props.allocType = cudaMemAllocationTypePinned;
+            props.location.type = cudaMemLocationTypeDevice;
+            props.location.id = device;
+            // (the first call may be one that a stream captures)
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            cudaError_t e = cudaMemPoolCreate(&pool, &props);
+            uint64_t keep = ~0ull;
+            if (e == cudaSuccess) e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            if (e != cudaSuccess) return e;
+            g_scratch_pool[device].store(pool, std::memory_order_release);
         }
-        configured[device].store(true, std::memory_order_relaxed);
     }
-    return cudaMallocAsync(p, bytes, s);
+    return cudaMallocFromPoolAsync(p, bytes, pool, s);
+}
+// unused blocks back to the system
+static void scratch_trim(int device) {
+    if (device < 0 || device >= 64) return;
+    if (cudaMemPool_t pool = g_scratch_pool[device].load(std::memory_order_acquire)) cudaMemPoolTrimTo(pool, 0);
 }
 
 }  // namespace ti
@@ -107,6 +126,7 @@ ti_status ti_shutdown(void) {
     for (int d = 0; d < n; ++d) {
         cudaMemPool_t pool;
         if (cudaDeviceGetDefaultMemPool(&pool, d) == cudaSuccess) cudaMemPoolTrimTo(pool, 0);
+        scratch_trim(d);
     }
     cudaGetLastError();
     return TI_OK;
@@ -147,8 +167,17 @@ ti_status ti_set_device(int device) {
 ti_status ti_malloc(int device, size_t bytes, void** ptr) {
     TI_CHECK(ptr, TI_ERR_INVALID, "ti_malloc: null out pointer");
     DeviceGuard g(device);
+    static std::atomic<bool> configured[64];
+    if (device >= 0 && device < 64 && !configured[device].load(std::memory_order_relaxed)) {
+        cudaMemPool_t pool;
+        if (cudaDeviceGetDefaultMemPool(&pool, device) == cudaSuccess) {
+            uint64_t thr = ~0ull;
+            cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &thr);
+        }
+        configured[device].store(true, std::memory_order_relaxed);
+    }
     void* p = nullptr;
-    cudaError_t e = pool_alloc(&p, bytes ? bytes : 1, device, (cudaStream_t)0);
+    cudaError_t e = cudaMallocAsync(&p, bytes ? bytes : 1, (cudaStream_t)0);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return fail(TI_ERR_OOM, "ti_malloc(%zu): %s", bytes, cudaGetErrorString(e));

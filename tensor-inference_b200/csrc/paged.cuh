@@ -241,8 +241,8 @@ TI_DEVICE_INLINE void tma_load_page(void* dst, const CUtensorMap* map, int row, 
         : "memory");
 }
 
-// stream-ordered memory of the device's pool, which keeps freed blocks for the next call (api.cpp)
-cudaError_t pool_alloc(void** p, size_t bytes, int device, cudaStream_t s);
+// stream-ordered memory of the library's pool on the device, which keeps freed blocks for the next call (api.cpp)
+cudaError_t scratch_alloc(void** p, size_t bytes, int device, cudaStream_t s);
 
 // both take their scratch from the pool; dev is the current device
 cudaError_t paged_decode_launch(const PagedAttn& p, int dev, cudaStream_t s);

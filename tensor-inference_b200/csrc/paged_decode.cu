@@ -689,7 +689,7 @@ cudaError_t paged_decode_launch(const PagedAttn& p, int dev, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     float* scratch = nullptr;
     const size_t rows = (size_t)ctas * 2 * a.rows;
-    e = pool_alloc(reinterpret_cast<void**>(&scratch), rows * (p.hd + 2) * sizeof(float), dev, s);
+    e = scratch_alloc(reinterpret_cast<void**>(&scratch), rows * (p.hd + 2) * sizeof(float), dev, s);
     if (e != cudaSuccess) return e;
     a.part_o = scratch;
     a.part_ml = scratch + rows * p.hd;

@@ -1151,7 +1151,7 @@ cudaError_t paged_prefill_launch(const PagedAttn& p, int dev, cudaStream_t s) {
     float* scratch = nullptr;
     const size_t n = (size_t)a.splits * p.r.n_tokens * p.n_heads;
     if (a.splits > 1) {
-        e = pool_alloc(reinterpret_cast<void**>(&scratch), n * (p.hd + 2) * sizeof(float), dev, s);
+        e = scratch_alloc(reinterpret_cast<void**>(&scratch), n * (p.hd + 2) * sizeof(float), dev, s);
         if (e != cudaSuccess) return e;
         a.part_o = scratch;
         a.part_ml = scratch + n * p.hd;

@@ -1,6 +1,9 @@
 """Attention over the paged cache at its edges: infinities and NaN that tokens see, weights that are small beside the
 largest, keys divided over CTAs under every mask, waits that give up."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -346,3 +349,54 @@ def test_pages_that_do_not_exist_are_zeros_that_take_weight(entry, max_len, hd, 
     q, f = queries(c, heads).abs(), forms(c, heads, **FORMS[form])
     ref, tol = attend(c, q, heads, **f)
     within(launch(c, c.dev(decode=entry == "decode"), q, heads, entry, f), ref, tol)
+
+
+# ------------------------------------------------------------------ scratch
+POOL = """
+import ctypes as C, sys
+sys.path[:0] = [%r, %r]
+import torch
+import ti_b200 as ti
+from paged_ref import Cache
+from test_gpu_paged_ops import queries, run_attention, within
+rt = C.CDLL("libcudart.so.12")
+def default_threshold():
+    pool, value = C.c_void_p(), C.c_uint64()
+    assert rt.cudaDeviceGetDefaultMemPool(C.byref(pool), 0) == 0
+    assert rt.cudaMemPoolGetAttribute(pool, 4, C.byref(value)) == 0  # cudaMemPoolAttrReleaseThreshold
+    return value.value
+torch.zeros(1, device="cuda")
+before = default_threshold()
+c = Cache([(1, 3000), (1, 40)], 1, 64, "bf16", seed=5)
+if sys.argv[1] == "captured":  # the process's first call, in a captured stream
+    d = c.dev(decode=True)
+    q = queries(c, 4).cuda()
+    out = torch.zeros_like(q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ti.check(ti.lib().ti_op_paged_decode(C.byref(d["kv"]), C.byref(d["batch"]), None, q.data_ptr(), 256, 4,
+                                             out.data_ptr(), 256, torch.cuda.current_stream().cuda_stream))
+    g.replay()
+    want, ref, tol = run_attention(c, q.cpu(), 4, "decode")
+    within(want, ref, tol)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+else:
+    out, ref, tol = run_attention(c, queries(c, 4), 4, "decode")
+    within(out, ref, tol)
+    p = Cache([(3, 3000)], 1, 64, "bf16", seed=5)
+    out, ref, tol = run_attention(p, queries(p, 4), 4, "prefill")  # keys divided: with scratch
+    within(out, ref, tol)
+assert default_threshold() == before, (before, default_threshold())
+ti.check(ti.lib().ti_shutdown())
+out, ref, tol = run_attention(c, queries(c, 4), 4, "decode")  # and the library stays usable
+within(out, ref, tol)
+"""
+
+
+@pytest.mark.parametrize("first", ["plain", "captured"])
+def test_scratch_leaves_the_default_pool_as_it_is(first):
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = POOL % (os.path.join(os.path.dirname(here), "tensor-inference_b200"), here)
+    r = subprocess.run([sys.executable, "-c", code, first], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0, r.stdout + r.stderr

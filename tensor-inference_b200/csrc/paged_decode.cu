@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         const CUtensorMap* tm = warp == kDecWarps ? &tk : &tv;
         const uint32_t half = warp == kDecWarps ? 0u : VOFF;
         int it = 0, issued = 0;
-        bool dead = false;  // a wait gave up: nothing more is requested
+        unsigned end = half == 0u ? (unsigned)a.p.stop_at : ~0u;  // first step not requested; 0 once a wait has given up
         segments([&](int, const SeqRange& x, int seg, int p0, int p1) {
             const int hk = seg / a.chunks;
             const int32_t* ids = x.row + x.pg0;
@@ -250,9 +250,11 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                     ahead = p + 32 + lane < p1 ? ids[p + 32 + lane] : 0;
                 }
                 const int id = __shfl_sync(0xffffffffu, cur, (i + lane) & 31);  // lane l: page p + l
-                if (half == 0u && it == a.p.stop_at) *stop = dead = true;
-                dead = dead || !__all_sync(0xffffffffu, pipe_wait(&empty[slot], ((it / NS) & 1) ^ 1, stop));
-                if (dead) continue;
+                if ((unsigned)it >= end || !__all_sync(0xffffffffu, pipe_wait(&empty[slot], ((it / NS) & 1) ^ 1, stop))) {
+                    *stop = 1;
+                    end = 0;
+                    continue;
+                }
                 // a page that does not exist reads as zeros: rows past the end of the pool
                 const int row = id >= 0 && id < a.p.r.n_pages ? (id * a.p.n_kv + hk) * kPageTokens : a.cache_rows;
                 const bool one = elect_one();
@@ -408,8 +410,8 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                 mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
                 mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
                 const float n0 = fmaxf(m0, mx0);
-                const float u0 = (n0 == -INFINITY ? 0.f : n0) - Elem<T>::kTop;
-                const float al0 = n0 == -INFINITY ? 0.f : ex2(m0 - n0);
+                const float w0 = n0 == -INFINITY ? 0.f : n0, u0 = w0 - Elem<T>::kTop;
+                const float al0 = ex2(m0 - w0);
                 m0 = n0;
                 float s0 = 0.f;
 #pragma unroll
@@ -426,8 +428,8 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
                     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
                     const float n1 = fmaxf(m1, mx1);
-                    const float u1 = (n1 == -INFINITY ? 0.f : n1) - Elem<T>::kTop;
-                    al1 = n1 == -INFINITY ? 0.f : ex2(m1 - n1);
+                    const float w1 = n1 == -INFINITY ? 0.f : n1, u1 = w1 - Elem<T>::kTop;
+                    al1 = ex2(m1 - w1);
                     m1 = n1;
                     float s1 = 0.f;
 #pragma unroll

@@ -819,11 +819,12 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             hi = INT32_MAX;
             pos = INT32_MAX / 2;
         }
-        // Capped scores lie within +-cap2, and bf16 has fp32's range: up to cap2 = 80 (a cap of 55) one m serves
-        // every row.  m as near the largest score as leaves the smallest p at 2^-120: p is at most 1 up to
-        // cap2 = 60 and at most 2^40 at 80, so products with V and their sums stay in range as well
-        const bool flat = CAP && !BIAS && Elem<T>::kUmmaFmt == 1 && cap2 <= 80.f;
-        float m = flat ? fminf(cap2, 120.f - cap2) : -INFINITY, l = 0.f;
+        // Capped scores lie within +-cap2, and bf16 has fp32's range: up to cap2 = 73 (a cap of 50.5) one m serves
+        // every row.  m as near the largest score as leaves the smallest p at 2^-100: p is at most 1 up to
+        // cap2 = 50 and at most 2^46 at 73.  With every score at an end of the cap, products with V keep a result's bits
+        // for values from 2^-40 (whose products are subnormal, with nine bits left) to 2^70
+        const bool flat = CAP && !BIAS && Elem<T>::kUmmaFmt == 1 && cap2 <= 73.f;
+        float m = flat ? fminf(cap2, 100.f - cap2) : -INFINITY, l = 0.f;
         for (int it = 0; it < nt; ++it) {
             const int b = NQ == 2 ? q : it & 1;
             const uint32_t n = NQ == 2 ? it : it >> 1;

@@ -278,6 +278,24 @@ def test_many_small_weights_beside_a_large_one(entry, new, hd, max_len, gap, dty
     within(launch(c, c.dev(decode=entry == "decode"), q, 2, entry, f), ref, tol)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("small", [1e-3, 1e-7, 1e-10])
+@pytest.mark.parametrize("entry", ["prefill", "decode"])
+def test_small_values_under_scores_at_the_low_end_of_a_cap(entry, small, hd):
+    c = Cache([(1, 200)] if entry == "decode" else [(30, 200)], 1, hd, "bf16", seed=42)
+    c.K[0] = torch.full_like(c.K[0], -12)
+    c.V[0] = c.V[0] * small
+    for p in range(13):
+        m, page = min(16, 200 - p * 16), int(c.table[c.rows[0], p])
+        c.k[page, :, :m] = c.K[0][p * 16:p * 16 + m].transpose(0, 1)
+        c.v[page, :, :m] = c.V[0][p * 16:p * 16 + m].transpose(0, 1)
+    q = torch.ones(c.tokens, 2, hd, dtype=torch.bfloat16)
+    for cap in (20.0, 30.0, 41.0, 42.0, 46.0, 50.0, 51.0, 55.0):
+        f = forms(c, 2, cap=cap)
+        ref, tol = attend(c, q, 2, **f)
+        within(launch(c, c.dev(decode=entry == "decode"), q, 2, entry, f), ref, tol, f"cap {cap}")
+
+
 # ------------------------------------------------------------------ waits that give up
 @pytest.mark.parametrize("hd, dtype", [(64, "bf16"), (128, "f16"), (256, "bf16")])
 @pytest.mark.parametrize("max_len", [0, 1 << 20])

@@ -859,7 +859,8 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 h = fma2(h, z, dup2(c0));
                 return fma2(h, v, add);
             };
-            bool small = false;  // capped scores within the polynomial's range
+            const int cl = lo - k0, ch = hi - k0;  // the row sees this thread's keys [cl, ch)
+            bool late = false;  // capped scores within the polynomial's range, which the exponentials' loop applies
             float mx = 0.f;
             // what becomes of x below stands for the scores ym x + yb (base 2)
             float ym = CAP || BIAS ? 1.f : scale2, yb = 0.f;
@@ -868,19 +869,26 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             const bool line = BIAS && __all_sync(0xffffffffu, slope2 > 1e-12f && min(hi, k0 + N) <= pos + 1);
             const float d0 = BIAS ? (float)(pos - k0) : 0.f;
             if constexpr (CAP) {
+                if (edge) {  // (what a row does not see must not take it out of the polynomial's range)
+#pragma unroll
+                    for (int c = 0; c < N; ++c) x[c] = c >= cl && c < ch ? x[c] : 0.f;
+                }
+                bool small;
                 if (flat) {
-                    small = !edge && __all_sync(0xffffffffu, reduce(max3, [](float v) { return fabsf(v); }) <= s_max);
+                    small = __all_sync(0xffffffffu, reduce(max3, [](float v) { return fabsf(v); }) <= s_max);
                 } else {
                     mx = row_max();
-                    small = !edge && __all_sync(0xffffffffu, mx <= s_max && reduce(min3, same) >= -s_max);
+                    small = __all_sync(0xffffffffu, mx <= s_max && reduce(min3, same) >= -s_max);
                 }
-                if (small && !BIAS) {
+                late = small && !BIAS && !edge;
+                if (late) {
                     if (!flat) mx = poly(make_float2(mx, 0.f), dup2(0.f)).x;  // monotonic: the maximum of the capped scores
                 } else if (small) {
                     const float b0 = -slope2 * d0;
 #pragma unroll
                     for (int c = 0; c < N; c += 2) {
-                        const float2 bias = line ? make_float2(fmaf(slope2, (float)c, b0), fmaf(slope2, (float)(c + 1), b0))
+                        const float2 bias = !BIAS ? dup2(0.f)
+                                            : line ? make_float2(fmaf(slope2, (float)c, b0), fmaf(slope2, (float)(c + 1), b0))
                                                  : make_float2(-slope2 * fabsf(d0 - (float)c), -slope2 * fabsf(d0 - (float)(c + 1)));
                         const float2 y = poly(make_float2(x[c], x[c + 1]), bias);
                         x[c] = y.x;
@@ -908,12 +916,11 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 }
             }
             if (edge) {
-                const int cl = lo - k0, ch = hi - k0;
 #pragma unroll
                 for (int c = 0; c < N; ++c) x[c] = c >= cl && c < ch ? x[c] : -INFINITY;
             }
             if (!flat) {
-                if (!CAP || BIAS || !small) mx = fmaf(row_max(), ym, yb);
+                if (!late) mx = fmaf(row_max(), ym, yb);
                 *xrow(it & 1, half) = mx;  // the other half's maximum
                 pair_bar();
                 mx = fmaxf(mx, *xrow(it & 1, half ^ 1));
@@ -976,7 +983,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                     if (NQ == 2 || h == 1) ready(h == 0 ? &p_half[b] : &p_full[b]);
                 }
             };
-            if (CAP && !BIAS && small) exps([&](float2 v) { return poly(v, mu); });
+            if (CAP && late) exps([&](float2 v) { return poly(v, mu); });
             else exps([&](float2 v) { return fma2(v, mm, mu); });
             l += sum.x + sum.y;
             if (kTurns && (q == 0 || it + 1 < nt)) turn_pass(q);

@@ -296,6 +296,41 @@ def test_small_values_under_scores_at_the_low_end_of_a_cap(entry, small, hd):
         within(launch(c, c.dev(decode=entry == "decode"), q, 2, entry, f), ref, tol, f"cap {cap}")
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("cap", [65.0, 300.0, 2500.0, 10000.0])
+@pytest.mark.parametrize("entry", ["prefill", "decode"])
+def test_scores_far_below_a_wide_cap_keep_their_bits(entry, cap, bias, hd):
+    # in tiles that rows see in part as in the others: tanh(u) is u to 2.9e-6 there, not cap - 2 cap / (e^2u + 1), which
+    # is off by cap 2^-21 however small u is (a scale of 1 and a cap of 10,000: 0.005)
+    heads = 2
+    c = Cache([(1, 300)] if entry == "decode" else [(150, 300)], 1, hd, "f16", seed=43, std=3.0 / hd ** 0.5)
+    q = queries(c, heads)
+    f = forms(c, heads, cap=cap, bias=bias, scale=1.0)
+    ref, _ = attend(c, q, heads, **f)
+    out = launch(c, c.dev(decode=entry == "decode"), q, heads, entry, f).cpu().double().numpy()
+    i = np.arange(300 - c.seqs[0][0], 300)[:, None]
+    j = np.arange(300)[None]
+    K, V, u = c.K[0][:, 0].double().numpy(), c.V[0][:, 0].double().numpy(), 2.0 ** -11
+    for h in range(heads):
+        qh = q[:, h].double().numpy()
+        z = cap * np.tanh(qh @ K.T / cap)
+        # fp32 products over hd terms; the polynomial, 2^-18 of the score, and its roundings; the exponential, 2^-16
+        dz = (hd + 8) * 2.0 ** -24 * (np.abs(qh) @ np.abs(K).T) + np.abs(z) * (2.0 ** -18 + 2.0 ** -22) + 2.0 ** -16
+        if bias:
+            far = f["slopes"][h] * np.abs(i - j)
+            z = z - far
+            dz = dz + far * 2.0 ** -22
+        z = np.where(j <= i, z, -np.inf)
+        w = np.exp(z - z.max(-1, keepdims=True))
+        w /= w.sum(-1, keepdims=True)
+        # a score off by dz scales its p by 1 + dz; the p that a row has besides are off by their own
+        off = w * np.where(j <= i, dz, 0)
+        tol = u * np.abs(ref[:, h]) * 1.01 + (u * 1.01) * (w @ np.abs(V)) + 1.01 * (off @ np.abs(V) + off.sum(-1, keepdims=True) * np.abs(ref[:, h]))
+        tol = tol + 2.0 ** -24
+        assert (np.abs(out[:, h] - ref[:, h]) <= tol).all(), (np.abs(out[:, h] - ref[:, h]) / tol).max()
+
+
 # ------------------------------------------------------------------ waits that give up
 @pytest.mark.parametrize("hd, dtype", [(64, "bf16"), (128, "f16"), (256, "bf16")])
 @pytest.mark.parametrize("max_len", [0, 1 << 20])

@@ -331,6 +331,34 @@ def test_scores_far_below_a_wide_cap_keep_their_bits(entry, cap, bias, hd):
         assert (np.abs(out[:, h] - ref[:, h]) <= tol).all(), (np.abs(out[:, h] - ref[:, h]) / tol).max()
 
 
+# ------------------------------------------------------------------ keys divided over CTAs
+LONG = {
+    "plain": {},
+    "cap": dict(cap=25.0),
+    "bias": dict(bias=True),
+    "window": dict(window=1700),
+    "prefix": dict(prefix=True),
+    "docs": dict(docs=1300),
+    "all": dict(cap=6.0, bias=True, window=2100, prefix=True, docs=2600, scale=0.2),
+}
+
+
+@pytest.mark.parametrize("form", LONG)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prefill_with_divided_keys_under_every_mask(hd, dtype, form):
+    # up to a dozen shares; sequences with fewer key tiles than shares, one of none, rows whose range misses shares
+    heads, nkv = 6, 2
+    c = Cache([(37, 2900), (5, 1100), (0, 64), (3, 140), (1, 1)], nkv, hd, dtype, seed=45, pad_tokens=2, spare_rows=1)
+    c.max_len = 1 << 20
+    f, q = forms(c, heads, **LONG[form]), queries(c, heads)
+    ref, tol = attend(c, q, heads, **f)
+    out = launch(c, c.dev(), q, heads, "prefill", f)
+    real = int(c.starts[-1])
+    within(out[:real], ref[:real], tol[:real])
+    assert (out[real:] == 3.0).all()
+
+
 # ------------------------------------------------------------------ waits that give up
 @pytest.mark.parametrize("hd, dtype", [(64, "bf16"), (128, "f16"), (256, "bf16")])
 @pytest.mark.parametrize("max_len", [0, 1 << 20])

@@ -152,10 +152,8 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const __grid_const
 namespace {
 
 template <class T, bool PAGED>
-void rope_launch_t(const RopeArgs& a, bool vec, int grid, size_t smem, cudaStream_t s) {
-    constexpr int V = 16 / sizeof(T);
-    if (vec) k_rope_append<T, V, PAGED><<<grid, kRopeThreads, smem, s>>>(a);
-    else k_rope_append<T, 1, PAGED><<<grid, kRopeThreads, smem, s>>>(a);
+const void* rope_func(bool vec) {
+    return vec ? (const void*)&k_rope_append<T, 16 / sizeof(T), PAGED> : (const void*)&k_rope_append<T, 1, PAGED>;
 }
 
 cudaError_t rope_launch(RopeArgs& a, int dtype, bool paged, int sms, cudaStream_t s) {
@@ -174,16 +172,12 @@ cudaError_t rope_launch(RopeArgs& a, int dtype, bool paged, int sms, cudaStream_
     const int per = kRopeThreads / a.tpt;
     const int grid = (a.r.n_tokens + per - 1) / per;
     const size_t smem = (size_t)per * a.rope.half * sizeof(float2);
-    if (dtype == TI_DTYPE_BF16) {
-        if (paged) rope_launch_t<__nv_bfloat16, true>(a, vec, grid, smem, s);
-        else rope_launch_t<__nv_bfloat16, false>(a, vec, grid, smem, s);
-    } else if (dtype == TI_DTYPE_F16) {
-        if (paged) rope_launch_t<__half, true>(a, vec, grid, smem, s);
-        else rope_launch_t<__half, false>(a, vec, grid, smem, s);
-    } else {
-        rope_launch_t<float, false>(a, vec, grid, smem, s);
-    }
-    return cudaGetLastError();
+    const void* f = dtype == TI_DTYPE_BF16  ? (paged ? rope_func<__nv_bfloat16, true>(vec) : rope_func<__nv_bfloat16, false>(vec))
+                    : dtype == TI_DTYPE_F16 ? (paged ? rope_func<__half, true>(vec) : rope_func<__half, false>(vec))
+                                            : rope_func<float, false>(vec);
+    // (its own status: cudaGetLastError would report an earlier call's error as this one's)
+    void* args[] = {&a};
+    return cudaLaunchKernel(f, dim3(grid), dim3(kRopeThreads), args, smem, s);
 }
 
 // ti_rope_axes -> kernel arguments, with the axis of every pair spelled out

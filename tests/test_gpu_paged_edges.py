@@ -432,6 +432,27 @@ def test_pages_that_do_not_exist_are_zeros_that_take_weight(entry, max_len, hd, 
     within(launch(c, c.dev(decode=entry == "decode"), q, heads, entry, f), ref, tol)
 
 
+# ------------------------------------------------------------------ errors
+def test_an_earlier_calls_error_is_not_this_ones():
+    c = Cache([(1, 20)], 1, 64, "bf16", seed=46)
+    d, x = c.dev(decode=True), torch.ones(1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    fr, pos = torch.ones(32, device="cuda"), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    r = ti.RopeAxes(rot_dim=64, inv_freq=fr.data_ptr(), n_axes=1, pos=pos.data_ptr(), pos_stride=1)
+    at, calls = x.data_ptr(), {
+        "rope": lambda: ti.lib().ti_op_rope_axes(ti.DTYPE_BF16, at, 128, at, 128, 1, 2, 64, C.byref(r), stream()),
+        "append": lambda: ti.lib().ti_op_kv_append(C.byref(d["kv"]), C.byref(d["batch"]), None, None, 0, at, 64, at, 64, 0,
+                                                   None, 0, stream()),
+        "prefill": lambda: ti.lib().ti_op_paged_prefill(C.byref(d["kv"]), C.byref(d["batch"]), None, at, 128, 2, at, 128,
+                                                        stream()),
+        "decode": lambda: ti.lib().ti_op_paged_decode(C.byref(d["kv"]), C.byref(d["batch"]), None, at, 128, 2, at, 128,
+                                                      stream()),
+    }
+    for name, call in calls.items():
+        assert ti.lib().ti_set_device(99) != 0
+        assert call() == 0, (name, ti.lib().ti_last_error().decode())
+    torch.cuda.synchronize()
+
+
 # ------------------------------------------------------------------ scratch
 POOL = """
 import ctypes as C, sys

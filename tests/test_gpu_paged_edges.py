@@ -432,6 +432,40 @@ def test_pages_that_do_not_exist_are_zeros_that_take_weight(entry, max_len, hd, 
     within(launch(c, c.dev(decode=entry == "decode"), q, heads, entry, f), ref, tol)
 
 
+# ------------------------------------------------------------------ large pools
+def test_pages_past_two_to_the_31_elements():
+    # pools of 2.3e9 elements each, the sequences' pages at their end
+    heads, nkv, hd, n_pages = 8, 8, 256, 70000
+    dec, pre = Cache([(1, 500), (1, 20)], nkv, hd, "bf16", seed=47), Cache([(90, 500), (20, 20)], nkv, hd, "bf16", seed=47)
+    pools = {w: torch.empty(n_pages, nkv, 16, hd, dtype=torch.bfloat16, device="cuda") for w in "kv"}
+    shift = n_pages - dec.n_pages
+    for entry, c in (("decode", dec), ("prefill", pre)):
+        f, q = forms(c, heads), queries(c, heads)
+        ref, tol = attend(c, q, heads, **f)
+        c.table = torch.where(c.table >= 0, c.table + shift, c.table)
+        d = c.dev(decode=entry == "decode")
+        for w in "kv":
+            pools[w][shift:] = d[w]
+        d["k"], d["v"] = pools["k"], pools["v"]
+        d["kv"].k_pages, d["kv"].v_pages, d["kv"].n_pages = pools["k"].data_ptr(), pools["v"].data_ptr(), n_pages
+        out = launch(c, d, q, heads, entry, f)
+        within(out, ref, tol)
+        put(c, d["v"], 0, 450, 3, 200, float("inf"))
+        want = np.zeros(ref.shape)
+        want[:c.seqs[0][0], 3, 200][sees(c, 0, 450, f)] = np.inf
+        same_odd_values(launch(c, d, q, heads, entry, f), want, ref, tol)
+        # and the append: new rows into the same slots
+        rows = torch.randn(c.tokens, 2, nkv, hd, device="cuda").bfloat16()
+        ti.check(ti.lib().ti_op_kv_append(C.byref(d["kv"]), C.byref(d["batch"]), None, None, 0, rows.data_ptr(),
+                                          2 * nkv * hd, rows.data_ptr() + 2 * nkv * hd, 2 * nkv * hd, 0, None, 0, stream()))
+        for s, (new, n) in enumerate(c.seqs):
+            at = torch.arange(n - new, n)
+            page = c.table[c.rows[s]][at // 16].long().cuda()
+            for i, w in enumerate("kv"):
+                t0 = int(c.starts[s])
+                assert torch.equal(d[w][page, :, (at % 16).cuda()], rows[t0:t0 + new, i])
+
+
 # ------------------------------------------------------------------ errors
 def test_an_earlier_calls_error_is_not_this_ones():
     c = Cache([(1, 20)], 1, 64, "bf16", seed=46)

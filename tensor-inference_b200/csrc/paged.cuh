@@ -89,8 +89,9 @@ TI_DEVICE_INLINE void finite_only(uint4& v) {
 TI_DEVICE_INLINE float odd_value(uint32_t kind) {
     return kind == 1 ? INFINITY : kind == 2 ? -INFINITY : __int_as_float(0x7fffffff);
 }
-// a partial output times its weight: an infinity counts even where its weight has come to zero
-TI_DEVICE_INLINE float join_add(float o, float v, float f) { return fabsf(v) == INFINITY ? o + v : fmaf(v, f, o); }
+// weight of a partial, 2^x for x <= 0, the smallest number there is instead of zero: an infinity in the partial then stays
+// one (and what is finite adds next to nothing)
+TI_DEVICE_INLINE float join_weight(float x) { return fmaxf(ex2(x), __int_as_float(1)); }
 
 // ------------------------------------------------------------------ warp-level products
 TI_DEVICE_INLINE void ldsm4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {

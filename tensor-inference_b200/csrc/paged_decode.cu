@@ -356,11 +356,9 @@ __global__ void __launch_bounds__(kDecThreads, 1)
             const int tok0 = (x.pg0 + p0 + st * CP) * kPageTokens;  // key of stage row 0
             const int rows = min(CP, p1 - p0 - st * CP) * kPageTokens;
             const int jlo = max(x.lo - tok0, 0), jhi = min(x.hi - tok0, rows);
-            if (!__all_sync(0xffffffffu, pipe_wait(&full[slot], (gi / NS) & 1, stop))) {
-                l0 = l1 = __int_as_float(0x7fffffff);  // keys are missing: the rows are NaN; and the slot is not handed back
-                continue;
-            }
-            if (j0 + 16 > jlo && j0 < jhi) {  // warp-uniform
+            const bool bad = !__all_sync(0xffffffffu, pipe_wait(&full[slot], (gi / NS) & 1, stop));
+            if (bad) l0 = l1 = __int_as_float(0x7fffffff);  // keys are missing: the rows are NaN; and the slot is not handed back
+            if (j0 + 16 > jlo && j0 < jhi && !bad) {  // warp-uniform
                 const bool edge = j0 < jlo || j0 + 16 > jhi;
                 if (edge) {
                     // unseen rows get probability 0: whatever their V holds must not enter
@@ -475,7 +473,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[slot]);
+            if (lane == 0 && !bad) mbar_arrive(&empty[slot]);
         }
 
         // ---- join the warps: every warp leaves its state, then every thread makes four of the outputs
@@ -616,7 +614,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_consta
         float l = 0.f;
         for (int c = lane; c < nc; c += 32) {
             const float2 x = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + row_of(c0 + c, r));
-            const float f = ex2(x.x - u);
+            const float f = join_weight(x.x - u);
             w[c * kDecRows + r] = f;
             l = fmaf(x.y, f, l);
         }
@@ -631,10 +629,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const __grid_consta
         for (int c = 0; c < nc; ++c) {
             const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + row_of(c0 + c, r) * HD + d));
             const float f = w[c * kDecRows + r];
-            o.x = join_add(o.x, v.x, f);
-            o.y = join_add(o.y, v.y, f);
-            o.z = join_add(o.z, v.z, f);
-            o.w = join_add(o.w, v.w, f);
+            o.x = fmaf(v.x, f, o.x);
+            o.y = fmaf(v.y, f, o.y);
+            o.z = fmaf(v.z, f, o.z);
+            o.w = fmaf(v.w, f, o.w);
         }
         out[e] = Elem<T>::from_f(o.x * inv[r]);
         out[e + 1] = Elem<T>::from_f(o.y * inv[r]);

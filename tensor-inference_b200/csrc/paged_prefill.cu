@@ -1086,10 +1086,10 @@ __global__ void __launch_bounds__(128) k_prefill_join(const __grid_constant__ Pr
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + r;
     const float2 x0 = lane < a.splits ? ml[lane * rows] : none, x1 = lane + 32 < a.splits ? ml[(lane + 32) * rows] : none;
     const float M = warp_max(fmaxf(x0.x, x1.x)), u = M == -INFINITY ? 0.f : M;
-    // (a split that saw nothing of the row did not write its output: -1, not read)
-    const float f0 = x0.x == -INFINITY && x0.y == 0.f ? -1.f : ex2(x0.x - u);
-    const float f1 = x1.x == -INFINITY && x1.y == 0.f ? -1.f : ex2(x1.x - u);
-    const float l = warp_sum(x0.y * fmaxf(f0, 0.f) + x1.y * fmaxf(f1, 0.f));
+    // a split that saw nothing of the row did not write its output (0: not read)
+    const float f0 = x0.x == -INFINITY && x0.y == 0.f ? 0.f : join_weight(x0.x - u);
+    const float f1 = x1.x == -INFINITY && x1.y == 0.f ? 0.f : join_weight(x1.x - u);
+    const float l = warp_sum(x0.y * f0 + x1.y * f1);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* out = reinterpret_cast<T*>(a.p.out) + (int64_t)t * a.p.out_stride + (int64_t)h * HD;
     const float* po = a.part_o + r * HD;
@@ -1098,9 +1098,9 @@ __global__ void __launch_bounds__(128) k_prefill_join(const __grid_constant__ Pr
 #pragma unroll 8
         for (int z = 0; z < a.splits; ++z) {
             const float f = __shfl_sync(0xffffffffu, z < 32 ? f0 : f1, z & 31);
-            const float2 v = f < 0.f ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(po + z * rows * HD + d);
-            o0 = join_add(o0, v.x, f);
-            o1 = join_add(o1, v.y, f);
+            const float2 v = f == 0.f ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(po + z * rows * HD + d);
+            o0 = fmaf(v.x, f, o0);
+            o1 = fmaf(v.y, f, o1);
         }
         out[d] = Elem<T>::from_f(o0 * inv);
         out[d + 1] = Elem<T>::from_f(o1 * inv);

@@ -859,7 +859,6 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 h = fma2(h, z, dup2(c0));
                 return fma2(h, v, add);
             };
-            const int cl = lo - k0, ch = hi - k0;  // the row sees this thread's keys [cl, ch)
             bool late = false;  // capped scores within the polynomial's range, which the exponentials' loop applies
             float mx = 0.f;
             // what becomes of x below stands for the scores ym x + yb (base 2)
@@ -870,6 +869,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             const float d0 = BIAS ? (float)(pos - k0) : 0.f;
             if constexpr (CAP) {
                 if (edge) {  // (what a row does not see must not take it out of the polynomial's range)
+                    const int cl = lo - k0, ch = hi - k0;
 #pragma unroll
                     for (int c = 0; c < N; ++c) x[c] = c >= cl && c < ch ? x[c] : 0.f;
                 }
@@ -916,6 +916,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
                 }
             }
             if (edge) {
+                const int cl = lo - k0, ch = hi - k0;
 #pragma unroll
                 for (int c = 0; c < N; ++c) x[c] = c >= cl && c < ch ? x[c] : -INFINITY;
             }

@@ -325,6 +325,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         q_seg = seg;
     };
     int it = 0, seg_no = 0;  // stages before this segment; segments before it
+    bool lost = false;       // a wait of this warp gave up
     segments([&](int s, const SeqRange& x, int seg, int p0, int p1) {
         const int hk = seg / a.chunks, h0 = hk * a.group + (seg % a.chunks) * kDecRows;
         const int G = min(kDecRows, (hk + 1) * a.group - h0);
@@ -356,9 +357,11 @@ __global__ void __launch_bounds__(kDecThreads, 1)
             const int tok0 = (x.pg0 + p0 + st * CP) * kPageTokens;  // key of stage row 0
             const int rows = min(CP, p1 - p0 - st * CP) * kPageTokens;
             const int jlo = max(x.lo - tok0, 0), jhi = min(x.hi - tok0, rows);
-            const bool bad = !__all_sync(0xffffffffu, pipe_wait(&full[slot], (gi / NS) & 1, stop));
-            if (bad) l0 = l1 = __int_as_float(0x7fffffff);  // keys are missing: the rows are NaN; and the slot is not handed back
-            if (j0 + 16 > jlo && j0 < jhi && !bad) {  // warp-uniform
+            // keys are missing once a wait has given up: the rows are NaN, and the slot is not handed back.  (For good: a slot's next
+            // phase but one has the parity that it shows already)
+            lost = lost || !__all_sync(0xffffffffu, pipe_wait(&full[slot], (gi / NS) & 1, stop));
+            if (lost) l0 = l1 = __int_as_float(0x7fffffff);
+            if (j0 + 16 > jlo && j0 < jhi && !lost) {  // warp-uniform
                 const bool edge = j0 < jlo || j0 + 16 > jhi;
                 if (edge) {
                     // unseen rows get probability 0: whatever their V holds must not enter
@@ -473,7 +476,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
                 }
             }
             __syncwarp();
-            if (lane == 0 && !bad) mbar_arrive(&empty[slot]);
+            if (lane == 0 && !lost) mbar_arrive(&empty[slot]);
         }
 
         // ---- join the warps: every warp leaves its state, then every thread makes four of the outputs

@@ -408,6 +408,25 @@ def test_decode_rows_are_nan_where_a_wait_gives_up(heads, lens, step, hd, dtype)
     assert torch.equal(launch(c, d, q, heads, "decode", f), clean)
 
 
+@pytest.mark.parametrize("hd, dtype, tokens", [(256, "bf16", 128), (128, "f16", 256), (64, "bf16", 512)])
+@pytest.mark.parametrize("step", [8, 9, 16])
+def test_decode_blocks_of_many_sequences_give_up_for_good(step, hd, dtype, tokens):
+    # sequences of eight steps each, several a block: later ones meet slots whose phase looks like one that has come
+    heads, n = 2, 1200
+    c = Cache([(1, tokens)] * n, 1, hd, dtype, seed=48)
+    d, f, q = c.dev(decode=True), forms(c, heads), queries(c, heads)
+    clean = launch(c, d, q, heads, "decode", f)
+    assert clean.isfinite().all()
+    try:
+        ti.check(ti.lib().ti_selftest_paged_stop(step))
+        out = launch(c, d, q, heads, "decode", f)
+    finally:
+        ti.check(ti.lib().ti_selftest_paged_stop(-1))
+    lost = out.isnan().all(-1)
+    assert lost.any() and not lost.all() and torch.equal(out[~lost], clean[~lost])
+    assert torch.equal(launch(c, d, q, heads, "decode", f), clean)
+
+
 # ------------------------------------------------------------------ pages that do not exist
 @pytest.mark.parametrize("form", ["plain", "cap", "bias", "all"])
 @pytest.mark.parametrize("hd, dtype", [(64, "f16"), (128, "bf16"), (256, "f16")])

@@ -822,7 +822,7 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
         // Capped scores lie within +-cap2, and bf16 has fp32's range: up to cap2 = 73 (a cap of 50.5) one m serves
         // every row.  m as near the largest score as leaves the smallest p at 2^-100: p is at most 1 up to
         // cap2 = 50 and at most 2^46 at 73.  With every score at an end of the cap, products with V keep a result's bits
-        // for values from 2^-40 (whose products are subnormal, with nine bits left) to 2^70
+        // for values from 2^-40 (whose products are subnormal, with nine bits left) to 2^60
         const bool flat = CAP && !BIAS && Elem<T>::kUmmaFmt == 1 && cap2 <= 73.f;
         float m = flat ? fminf(cap2, 100.f - cap2) : -INFINITY, l = 0.f;
         for (int it = 0; it < nt; ++it) {
@@ -868,15 +868,15 @@ __global__ void __launch_bounds__(PreCfg<HD>::THREADS, 1)
             const bool line = BIAS && __all_sync(0xffffffffu, slope2 > 1e-12f && min(hi, k0 + N) <= pos + 1);
             const float d0 = BIAS ? (float)(pos - k0) : 0.f;
             if constexpr (CAP) {
-                if (edge) {  // (what a row does not see must not take it out of the polynomial's range)
-                    const int cl = lo - k0, ch = hi - k0;
-#pragma unroll
-                    for (int c = 0; c < N; ++c) x[c] = c >= cl && c < ch ? x[c] : 0.f;
-                }
                 bool small;
-                if (flat) {
-                    small = __all_sync(0xffffffffu, reduce(max3, [](float v) { return fabsf(v); }) <= s_max);
+                if (flat) {  // (caps up to 50.5: edge tiles may take the exponential form, off by 2^-15 at most)
+                    small = !edge && __all_sync(0xffffffffu, reduce(max3, [](float v) { return fabsf(v); }) <= s_max);
                 } else {
+                    if (edge) {  // (what a row does not see must not take it out of the polynomial's range)
+                        const int cl = lo - k0, ch = hi - k0;
+#pragma unroll
+                        for (int c = 0; c < N; ++c) x[c] = c >= cl && c < ch ? x[c] : 0.f;
+                    }
                     mx = row_max();
                     small = __all_sync(0xffffffffu, mx <= s_max && reduce(min3, same) >= -s_max);
                 }

@@ -4,6 +4,7 @@ import ctypes as C
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -449,6 +450,41 @@ def test_pages_that_do_not_exist_are_zeros_that_take_weight(entry, max_len, hd, 
     q, f = queries(c, heads).abs(), forms(c, heads, **FORMS[form])
     ref, tol = attend(c, q, heads, **f)
     within(launch(c, c.dev(decode=entry == "decode"), q, heads, entry, f), ref, tol)
+
+
+# ------------------------------------------------------------------ calls at once
+def test_two_host_threads_on_streams_of_their_own():
+    # divided and joined calls, with scratch, one of them settling odd values: every result as when made alone
+    heads = 4
+    jobs = []
+    for seed, (entry, seqs) in enumerate([("decode", [(1, 5000), (1, 70)]), ("prefill", [(40, 3000), (130, 130)])]):
+        c = Cache(seqs, 1, 128, "bf16", seed=50 + seed)
+        d, f, q = c.dev(decode=entry == "decode"), forms(c, heads, cap=20.0), queries(c, heads).cuda()
+        put(c, d["v"], 0, 60, 0, 9, float("inf"))
+        put(c, d["v"], 1, 65, 0, 11, float("nan"))
+        fm = ti.AttnForm(softcap=20.0)
+        jobs.append((c, d, f, q, entry, fm, launch(c, d, q, heads, entry, f).view(torch.int16).clone()))
+    failed = []
+
+    def work(c, d, f, q, entry, fm, want):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            outs = [torch.zeros(c.tokens, heads, 128, dtype=torch.bfloat16, device="cuda") for _ in range(30)]
+            for out in outs:
+                st = getattr(ti.lib(), f"ti_op_paged_{entry}")(C.byref(d["kv"]), C.byref(d["batch"]), C.byref(fm), q.data_ptr(),
+                                                               heads * 128, heads, out.data_ptr(), heads * 128, s.cuda_stream)
+                if st != 0:
+                    failed.append((entry, st))
+        s.synchronize()
+        failed.extend(entry for out in outs if not torch.equal(out.view(torch.int16), want))
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=job) for job in jobs for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
 
 
 # ------------------------------------------------------------------ large pools

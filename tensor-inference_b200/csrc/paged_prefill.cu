@@ -294,7 +294,8 @@ TI_DEVICE_INLINE void settle_odd(const PreArgs& a, uint8_t* smem, uint32_t tmem,
     };
     // (the K and V stages are free: every copy has landed and every MMA is done)
     uint32_t* planes = reinterpret_cast<uint32_t*>(smem + L.k);  // odd values of a tile: [+inf or NaN, -inf or NaN][HD][BN] bits
-    uint32_t* open = planes + 2 * HD * W;                        // outputs to compute again: [HD/32][rows]
+    uint32_t* dims = planes + 2 * HD * W;                        // dimensions with any: [HD/32]
+    uint32_t* open = dims + KW;                                  // outputs to compute again: [HD/32][rows]
     bool redo = false;
     {
         const int half = (warp >> 2) & 1;
@@ -304,7 +305,7 @@ TI_DEVICE_INLINE void settle_odd(const PreArgs& a, uint8_t* smem, uint32_t tmem,
 #pragma unroll
         for (int w = 0; w < HW; ++w) seen[0][w] = seen[1][w] = 0;
         auto clear = [&] {
-            for (int i = tid; i < 2 * HD * W; i += TH) planes[i] = 0;
+            for (int i = tid; i < 2 * HD * W + KW; i += TH) planes[i] = 0;  // (and dims)
             softmax_or<TH>(false);
         };
         clear();
@@ -317,6 +318,9 @@ TI_DEVICE_INLINE void settle_odd(const PreArgs& a, uint8_t* smem, uint32_t tmem,
                 const uint32_t odd = odd_kinds<T>(value_at(a.p.v_pages, k0 + r, d));
                 if (odd == 0) continue;
                 found = true;
+                uint32_t which = 0;
+                for (int e = 0; e < 8; ++e) which |= (uint32_t)((odd >> (2 * e) & 3u) != 0) << e;
+                atomicOr(&dims[d / 32], which << (d % 32));
                 for (int e = 0; e < 16; ++e)
                     if (odd >> e & 1u) atomicOr(&planes[((e & 1) * HD + d + e / 2) * W + r / 32], 1u << (r % 32));
             }
@@ -328,17 +332,19 @@ TI_DEVICE_INLINE void settle_odd(const PreArgs& a, uint8_t* smem, uint32_t tmem,
                 mask[w] = (b1 == 32 ? ~0u : (1u << b1) - 1u) & ~(b0 == 32 ? ~0u : (1u << b0) - 1u);
             }
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
+            for (int w = 0; w < HW; ++w)
+#pragma unroll 1
+                for (uint32_t left = dims[half * HW + w]; left; left &= left - 1) {
+                    const int b = __ffs(left) - 1;
 #pragma unroll
-                for (int w = 0; w < HW; ++w)
-#pragma unroll 4
-                    for (int b = 0; b < 32; ++b) {
+                    for (int p = 0; p < 2; ++p) {
                         const uint32_t* plane = planes + (p * HD + half * (HD / 2) + w * 32 + b) * W;
                         uint32_t any = 0;
 #pragma unroll
                         for (int k = 0; k < W; ++k) any |= plane[k] & mask[k];
                         seen[p][w] |= (uint32_t)(any != 0) << b;
                     }
+                }
             softmax_or<TH>(false);
             clear();
         }
@@ -372,7 +378,7 @@ TI_DEVICE_INLINE void settle_odd(const PreArgs& a, uint8_t* smem, uint32_t tmem,
     constexpr int KT = 64, NT = 8;  // keys of a tile, 8-dim columns
     uint8_t* kt = smem + L.v;       // [HD/64][KT][64], 128-byte swizzle
     uint8_t* vt = kt + KT * HD * 2;  // [KT][64], swizzled
-    static_assert(KT * HD * 2 + KT * 128 <= C::NS * C::KBYTES && 2 * HD * W * 4 + KW * C::ROWS * 4 <= C::NS * C::KBYTES, "fits the stages");
+    static_assert(KT * HD * 2 + KT * 128 <= C::NS * C::KBYTES && (2 * HD * W + KW * (1 + C::ROWS)) * 4 <= C::NS * C::KBYTES, "fits the stages");
     const int gq = lane >> 2, qq = lane & 3, row0 = warp * 16;
     const Row rows[2] = {row_of<HD>(a, rt, hk, row0 + gq, n_keys), row_of<HD>(a, rt, hk, row0 + gq + 8, n_keys)};
     float slope[2];
